@@ -43,6 +43,15 @@ SIGNATURES = {
     "dsa_index_cache_write": (_c_int, [_ptr, _c_int, _c_i64, _ptr, _ptr, _c_int, _c_int, _ptr, _ptr]),
     "dsa_kv_cache_append": (_c_int, [_ptr, _c_i64, _ptr, _c_i64, _ptr, _ptr, _ptr, _c_int, _c_i64,
                                      _ptr, _ptr]),
+    "dsa_paged_attn_workspace_bytes": (_c_size, [_c_int] * 5),
+    "dsa_paged_attn": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_i64, _c_float, _ptr, _ptr, _ptr, _c_i64,
+                                _ptr, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr, _c_size, _ptr, _ptr]),
+    "dsa_cache_evict": (_c_int, [_ptr, _c_i64, _ptr, _ptr, _c_i64, _ptr, _c_i64, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                 _c_i64, _ptr, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                 _ptr, _ptr]),
+    "dsa_rotary_append": (_c_int, [_ptr, _c_i64, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _c_int, _ptr,
+                                   ctypes.c_uint64, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_i64, _ptr,
+                                   _ptr]),
     "dsa_decode_step_host": (_c_int, [_ptr]),
     "dsa_peer_slab_create": (_c_int, [_c_size, _ptr, _ptr]),
     "dsa_peer_slab_open": (_c_int, [_ptr, _ptr]),

@@ -5,6 +5,8 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "paged_attn.cuh"
+#include "tmap.cuh"
 
 namespace dsa {
 cudaError_t launch_indexer_score_simt(const void*, const void*, const float*, const int32_t*,
@@ -41,6 +43,16 @@ cudaError_t launch_index_cache_write(const void*, int, int64_t, const int32_t*, 
 cudaError_t launch_kv_cache_append(const void*, int64_t, const void*, int64_t, const int32_t*, void*,
                                    void*, int, int64_t, int32_t*, cudaStream_t);
 size_t att_workspace_bytes(int tokens, int splits);
+int paged_block_rows(int rows);
+cudaError_t launch_paged_attn_mma(const PagedArgs&, const void*, const void*, cudaStream_t);
+cudaError_t launch_paged_join(const PagedArgs&, cudaStream_t);
+cudaError_t launch_paged_weights(const PagedArgs&, const float*, int64_t, float*, int64_t, cudaStream_t);
+cudaError_t launch_cache_evict(const float*, int64_t, const int32_t*, const int32_t*, int64_t, const int32_t*, int64_t, void*,
+                               void*, void*, int32_t*, float*, int64_t, int32_t*, int64_t, int, int, int, int, int, int,
+                               int32_t*, cudaStream_t);
+cudaError_t launch_rotary_append(const void*, int64_t, int64_t, const void*, int64_t, const void*, int64_t, const int32_t*,
+                                 int64_t, const float*, uint64_t, int, const int32_t*, void*, void*, void*, int, int, int64_t,
+                                 int32_t*, cudaStream_t);
 }  // namespace dsa
 
 namespace {
@@ -403,6 +415,129 @@ int dsa_kv_cache_append(const void* ckv, int64_t ckv_stride, const void* kpe, in
   return static_cast<int>(dsa::launch_kv_cache_append(ckv, ckv_stride, kpe, kpe_stride, slots,
                                                       ckv_cache, kpe_cache, tokens, num_slots,
                                                       status_dev, static_cast<cudaStream_t>(stream)));
+}
+
+// ---- dense attention over the paged caches, eviction from them, rotary append to them ----------
+static bool paged_shape_ok(int batch, int tokens, int heads, int max_pages) {
+  return batch >= 0 && batch <= 65535 && tokens >= 1 && heads >= 1 && heads <= 128 && (int64_t)tokens * heads <= 65536 &&
+         max_pages >= 1 && max_pages <= DSA_PAGED_MAX_PAGES;
+}
+// Ranges that the tiles are cut into: a CTA per SM over all row blocks, so that the blocks of one request walk its
+// pages at the same time and share them through L2.
+static int paged_ranges(int batch, int blocks, int max_pages) {
+  int x = dsa::sm_count() / blocks;
+  const int64_t tiles = (int64_t)batch * max_pages;
+  if (x > tiles) x = (int)tiles;
+  if (x > dsa::kPagedMaxRanges) x = dsa::kPagedMaxRanges;
+  return x < 1 ? 1 : x;
+}
+static int paged_blocks(int rows) { return (rows + dsa::paged_block_rows(rows) - 1) / dsa::paged_block_rows(rows); }
+static size_t paged_part_bytes(int batch, int rows, int max_pages) {
+  const int blocks = paged_blocks(rows);
+  return round256((size_t)paged_ranges(batch, blocks, max_pages) * blocks * 2 * dsa::paged_part_floats(dsa::paged_block_rows(rows)) * 4);
+}
+
+size_t dsa_paged_attn_workspace_bytes(int batch, int tokens_per_request, int heads, int max_pages, int with_weights) {
+  if (batch <= 0 || !paged_shape_ok(batch, tokens_per_request, heads, max_pages)) return 256;
+  const int rows = tokens_per_request * heads;
+  size_t n = paged_part_bytes(batch, rows, max_pages);
+  if (with_weights)
+    n += (size_t)batch * max_pages * paged_blocks(rows) * dsa::paged_block_rows(rows) * dsa::kPage * sizeof(float);
+  return n;
+}
+
+int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const void* kpe, const int32_t* seq_lens,
+                   const int32_t* block_table, int64_t block_table_stride, float sm_scale, void* out, float* lse,
+                   const float* token_weights, int64_t token_weights_stride, float* new_token_weights,
+                   int64_t new_token_weights_stride, int batch, int tokens_per_request, int heads, int num_pages,
+                   int max_pages, void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
+  if (batch == 0) return DSA_OK;
+  if (!q_nope || !q_pe || !ckv || !kpe || !seq_lens || !block_table || !out || !lse || !workspace)
+    return DSA_ERR_NULL_POINTER;
+  if (!paged_shape_ok(batch, tokens_per_request, heads, max_pages) || num_pages <= 0 ||
+      num_pages > DSA_PAGED_MAX_PAGES || block_table_stride < 0 || (token_weights && !new_token_weights))
+    return DSA_ERR_BAD_SHAPE;
+  const int64_t width = (int64_t)max_pages * dsa::kPage;
+  if (new_token_weights && (new_token_weights_stride < width || (token_weights && token_weights_stride < width)))
+    return DSA_ERR_BAD_SHAPE;
+  if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(out) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return DSA_ERR_MISALIGNED;
+  if (workspace_bytes < dsa_paged_attn_workspace_bytes(batch, tokens_per_request, heads, max_pages, new_token_weights != nullptr))
+    return DSA_ERR_WORKSPACE_TOO_SMALL;
+  const int rows = tokens_per_request * heads;
+  dsa::PagedArgs a = {};
+  a.q_nope = static_cast<const __nv_bfloat16*>(q_nope);
+  a.q_pe = static_cast<const __nv_bfloat16*>(q_pe);
+  a.seq_lens = seq_lens;
+  a.block_table = block_table;
+  a.table_stride = block_table_stride;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.part = static_cast<float*>(workspace);
+  a.logits = new_token_weights ? reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_part_bytes(batch, rows, max_pages))
+                               : nullptr;
+  a.status = status_dev;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.batch = batch;
+  a.max_pages = max_pages;
+  a.num_pages = num_pages;
+  a.rows = rows;
+  a.heads = heads;
+  a.tokens = tokens_per_request;
+  a.block_rows = dsa::paged_block_rows(rows);
+  a.grid_x = paged_ranges(batch, paged_blocks(rows), max_pages);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = dsa::launch_paged_attn_mma(a, ckv, kpe, s);
+  if (e == cudaSuccess && a.grid_x > 1) e = dsa::launch_paged_join(a, s);
+  if (e == cudaSuccess && new_token_weights)
+    e = dsa::launch_paged_weights(a, token_weights, token_weights_stride, new_token_weights, new_token_weights_stride, s);
+  return static_cast<int>(e);
+}
+
+int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, const int32_t* seq_lens,
+                    const int32_t* block_table, int64_t block_table_stride, const int32_t* new_block_table,
+                    int64_t new_block_table_stride, void* ckv, void* kpe, void* k_index_cache, int32_t* new_seq_lens,
+                    float* new_token_weights, int64_t new_token_weights_stride, int32_t* kept, int64_t kept_stride, int batch,
+                    int max_pages, int new_max_pages, int num_pages, int budget, int keep_first, int keep_last,
+                    int32_t* status_dev, void* stream) {
+  if (batch == 0) return DSA_OK;
+  if (!token_weights || !seq_lens || !block_table || !new_block_table || !ckv || !kpe || !new_seq_lens || !new_token_weights ||
+      !kept)
+    return DSA_ERR_NULL_POINTER;
+  const int64_t width = (int64_t)max_pages * dsa::kPage, most = width < budget ? width : budget;
+  if (batch < 0 || batch > 65535 || max_pages < 1 || max_pages > DSA_PAGED_MAX_PAGES || num_pages <= 0 ||
+      num_pages > DSA_PAGED_MAX_PAGES || budget < 1 || keep_first < 0 || keep_last < 0 ||
+      (int64_t)keep_first + keep_last > budget || (int64_t)new_max_pages * dsa::kPage < most || token_weights_stride < width ||
+      new_token_weights_stride < budget || kept_stride < budget || block_table_stride < 0 || new_block_table_stride < 0)
+    return DSA_ERR_BAD_SHAPE;
+  if (!aligned16(ckv) || !aligned16(kpe) || !aligned16(k_index_cache)) return DSA_ERR_MISALIGNED;
+  return static_cast<int>(dsa::launch_cache_evict(
+      token_weights, token_weights_stride, seq_lens, block_table, block_table_stride, new_block_table, new_block_table_stride,
+      ckv, kpe, k_index_cache, new_seq_lens, new_token_weights, new_token_weights_stride, kept, kept_stride, batch, max_pages,
+      num_pages, budget, keep_first, keep_last, status_dev, static_cast<cudaStream_t>(stream)));
+}
+
+int dsa_rotary_append(const void* q_pe, int64_t q_token_stride, int64_t q_head_stride, const void* ckv, int64_t ckv_stride,
+                      const void* kpe, int64_t kpe_stride, const int32_t* positions, int64_t positions_stride, int axes,
+                      const float* inv_freq, uint64_t pair_axes, int interleaved, const int32_t* slots, void* q_out,
+                      void* ckv_cache, void* kpe_cache, int tokens, int heads, int64_t num_slots, int32_t* status_dev,
+                      void* stream) {
+  if (tokens == 0) return DSA_OK;
+  if (!q_pe || !ckv || !kpe || !positions || !inv_freq || !slots || !q_out || !ckv_cache || !kpe_cache)
+    return DSA_ERR_NULL_POINTER;
+  if (tokens < 0 || heads < 1 || heads > 128 || axes < 1 || axes > 4 || num_slots <= 0 || positions_stride < tokens ||
+      ckv_stride < dsa::kCkv || kpe_stride < dsa::kKpe || q_token_stride < dsa::kKpe || q_head_stride < dsa::kKpe)
+    return DSA_ERR_BAD_SHAPE;
+  for (int i = 0; i < dsa::kKpe / 2; ++i)
+    if ((int)((pair_axes >> (2 * i)) & 3u) >= axes) return DSA_ERR_BAD_SHAPE;
+  if (!aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(q_out) || !aligned16(ckv_cache) ||
+      !aligned16(kpe_cache) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0 || ckv_stride % 8 != 0 || kpe_stride % 8 != 0)
+    return DSA_ERR_MISALIGNED;
+  return static_cast<int>(dsa::launch_rotary_append(q_pe, q_token_stride, q_head_stride, ckv, ckv_stride, kpe, kpe_stride,
+                                                    positions, positions_stride, inv_freq, pair_axes, interleaved, slots, q_out,
+                                                    ckv_cache, kpe_cache, tokens, heads, num_slots, status_dev,
+                                                    static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -53,6 +53,18 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory spans of two tensors meet (from the first element to the last, gaps included)."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        first = t.data_ptr()
+        return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    a0, a1 = span(a)
+    b0, b1 = span(b)
+    return a0 < b1 and b0 < a1
+
+
 STATUS_BITS = {
     0x1: "a bounded device-side wait timed out",
     0x2: "block_table entry outside [0, num_pages)",

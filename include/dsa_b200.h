@@ -191,6 +191,81 @@ int dsa_kv_cache_append(const void* ckv, int64_t ckv_stride, const void* kpe, in
                         int64_t num_slots, int32_t* status_dev, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Dense MLA attention of every request's newest tokens over its whole paged cache (no counterpart in the
+ * reference, whose attention reads a list of slots): layers without an indexer, contexts too short for one, drafted
+ * tokens.  The cache layout is that of dsa_sparse_attn, addressed by the indexer's block table.
+ *
+ *   q_nope  [batch*tokens_per_request,heads,512] bf16   q_pe [..,heads,64] bf16   (contiguous; heads 1..128)
+ *   ckv     [num_pages,64,512] bf16      kpe  [num_pages,64,64] bf16
+ *   seq_lens [batch] int32 cached tokens, the new ones among them; block_table [batch,max_pages] int32, row stride
+ *           `block_table_stride` elements (0 = every request shares one row)
+ *   out     [batch*tokens_per_request,heads,512] bf16   lse [..,heads] fp32 (base-2 log-sum-exp)
+ * Token i of a request's n new ones stands at position seq_len - n + i and sees the positions up to its own; one
+ * that stands before the request's beginning sees nothing and gets out = 0 and lse = -inf.  Positions at or
+ * behind seq_len may hold anything; those in front of it must be finite.  seq_len is taken within
+ * [0, 64 * max_pages].  A page id outside [0, num_pages) is left out of the sums (DSA_STATUS_BAD_PAGE).
+ *   new_token_weights (may be NULL) [batch,>= 64*max_pages] fp32, row stride in elements: for every pos < seq_len
+ *           new_token_weights[b,pos] = token_weights[b,pos] + the sum over the request's query rows (tokens and
+ *           heads) of their softmax weight of that position; token_weights NULL = zeros; the two may be one
+ *           buffer.  Entries at or behind seq_len are left as they were.
+ *   workspace >= dsa_paged_attn_workspace_bytes(...) bytes, 256-byte aligned, any contents; calls that may
+ *           overlap need workspaces of their own.
+ * max_pages, num_pages <= DSA_PAGED_MAX_PAGES; tokens_per_request * heads <= 65536.
+ * ------------------------------------------------------------------------------------------- */
+#define DSA_PAGED_MAX_PAGES (1 << 24)
+
+size_t dsa_paged_attn_workspace_bytes(int batch, int tokens_per_request, int heads, int max_pages,
+                                      int with_weights);
+
+int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const void* kpe,
+                   const int32_t* seq_lens, const int32_t* block_table, int64_t block_table_stride,
+                   float sm_scale, void* out, float* lse, const float* token_weights,
+                   int64_t token_weights_stride, float* new_token_weights, int64_t new_token_weights_stride,
+                   int batch, int tokens_per_request, int heads, int num_pages, int max_pages, void* workspace,
+                   size_t workspace_bytes, int32_t* status_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Eviction from the paged caches by accumulated attention weight (no counterpart in the reference).
+ *   token_weights [batch,>= 64*max_pages] fp32, row stride in elements (what dsa_paged_attn accumulates)
+ * A request of at most `budget` tokens keeps them all; a longer one keeps its first `keep_first` positions, its
+ * last `keep_last`, and of the others the heaviest (equal weights: the lower position; -inf and NaN lowest),
+ * `budget` in all.  Kept tokens stay in order: token j moves from its old slot to position j of the pages of
+ * new_block_table[b], its ckv and kpe rows and, where k_index_cache is not NULL, its index key and scale.
+ *   new_seq_lens [batch] int32 = min(seq_len, budget)
+ *   new_token_weights [batch,budget] fp32, kept [batch,budget] int32 (old positions), row strides in elements; behind
+ *   the last kept token 0 and -1.
+ * The old pages are only read.  A new page must not be an old page that a request of the call still reads
+ * from, unless every kept token on it keeps its place (a request within the budget may pass its old row and
+ * nothing moves), nor stand twice in new_block_table: such moves race.  The outputs must not overlap the inputs.
+ * Page ids outside [0, num_pages) are skipped (DSA_STATUS_BAD_PAGE).
+ * ------------------------------------------------------------------------------------------- */
+int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, const int32_t* seq_lens,
+                    const int32_t* block_table, int64_t block_table_stride, const int32_t* new_block_table,
+                    int64_t new_block_table_stride, void* ckv, void* kpe, void* k_index_cache,
+                    int32_t* new_seq_lens, float* new_token_weights, int64_t new_token_weights_stride,
+                    int32_t* kept, int64_t kept_stride, int batch, int max_pages, int new_max_pages,
+                    int num_pages, int budget, int keep_first, int keep_last, int32_t* status_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions with one to four axes (time, height, width ..) on q_pe and on the new keys, and the append of
+ * the keys: the producer of dsa_paged_attn's and dsa_sparse_attn's inputs (no counterpart in the reference, whose
+ * inputs arrive rotated).
+ *   angle[t,i] = positions[axis of pair i, t] * inv_freq[i], in 64 bits; axis of pair i = bits 2i, 2i+1 of `pair_axes`
+ *   q_pe  [tokens,heads,64] bf16, token and head strides in elements (multiples of 8)
+ *   ckv [tokens,512], kpe [tokens,64] bf16, row strides in elements (multiples of 8)
+ *   positions [axes,tokens] int32, row stride in elements; inv_freq [32] fp32
+ *   interleaved 1: the pairs are the neighbours (2i, 2i+1); 0: (i, i + 32)
+ *   q_out [tokens,heads,64] bf16 contiguous (may be q_pe where that is contiguous) receives the rotated queries of
+ *   every token; ckv_cache / kpe_cache [num_slots,512 / 64] receive ckv[t] and the rotated kpe[t] at slot slots[t]
+ *   (-1 = not cached, as for dsa_kv_cache_append, which also says what bad and equal slots do).
+ * ------------------------------------------------------------------------------------------- */
+int dsa_rotary_append(const void* q_pe, int64_t q_token_stride, int64_t q_head_stride, const void* ckv,
+                      int64_t ckv_stride, const void* kpe, int64_t kpe_stride, const int32_t* positions,
+                      int64_t positions_stride, int axes, const float* inv_freq, uint64_t pair_axes,
+                      int interleaved, const int32_t* slots, void* q_out, void* ckv_cache, void* kpe_cache,
+                      int tokens, int heads, int64_t num_slots, int32_t* status_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * One decode step with HOST buffers: copies in, dsa_indexer_topk, dsa_sparse_attn over the
  * indexer's own indices, copies out, synchronised on return.  No counterpart in the reference,
  * whose callers pass CUDA tensors (kbench/flashinfer.py:109-120); it replaces the nine copies and
