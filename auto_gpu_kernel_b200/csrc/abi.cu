@@ -43,8 +43,8 @@ cudaError_t launch_index_cache_write(const void*, int, int64_t, const int32_t*, 
 cudaError_t launch_kv_cache_append(const void*, int64_t, const void*, int64_t, const int32_t*, void*,
                                    void*, int, int64_t, int32_t*, cudaStream_t);
 size_t att_workspace_bytes(int tokens, int splits);
-int paged_block_rows(int rows);
 cudaError_t launch_paged_attn_mma(const PagedArgs&, const void*, const void*, cudaStream_t);
+cudaError_t launch_paged_attn_tc(const PagedArgs&, const void*, const void*, cudaStream_t);
 cudaError_t launch_paged_join(const PagedArgs&, cudaStream_t);
 cudaError_t launch_paged_weights(const PagedArgs&, const float*, int64_t, float*, int64_t, cudaStream_t);
 cudaError_t launch_cache_evict(const float*, int64_t, const int32_t*, const int32_t*, int64_t, const int32_t*, int64_t, void*,
@@ -488,7 +488,7 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
   a.block_rows = dsa::paged_block_rows(rows);
   a.grid_x = paged_ranges(batch, paged_blocks(rows), max_pages);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = dsa::launch_paged_attn_mma(a, ckv, kpe, s);
+  cudaError_t e = a.block_rows == 64 ? dsa::launch_paged_attn_tc(a, ckv, kpe, s) : dsa::launch_paged_attn_mma(a, ckv, kpe, s);
   if (e == cudaSuccess && a.grid_x > 1) e = dsa::launch_paged_join(a, s);
   if (e == cudaSuccess && new_token_weights)
     e = dsa::launch_paged_weights(a, token_weights, token_weights_stride, new_token_weights, new_token_weights_stride, s);

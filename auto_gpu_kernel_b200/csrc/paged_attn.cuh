@@ -32,6 +32,10 @@ struct PagedArgs {
 
 constexpr int kPagedMaxRanges = 512;
 
+// Query rows that a CTA takes at once, from the rows of a request: 16 or 32 by warp-level products (one or two row
+// groups per page), 64 by tcgen05.
+inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
 __host__ __device__ inline int paged_len(int len, int max_pages) {
   const int64_t most = (int64_t)max_pages * kPage;
   return len < 0 ? 0 : ((int64_t)len > most ? (int)most : len);
@@ -41,8 +45,8 @@ __host__ __device__ inline int paged_tiles(int len, int max_pages) {
   return n < 1 ? 1 : n;
 }
 
-// Partial results: per (row block, range, which) a [rows of the block][512] fp32 accumulator, then its running
-// maxima and sums.  `which` is 1 for the segment a request begins with and 0 for the ones that follow: a range
+// Partial results: per (row block, range, which) a [rows of the block][512] fp32 accumulator ([512][64] for blocks of
+// 64 rows), then its running maxima and sums.  `which` is 1 for the segment a request begins with and 0 for the ones that follow: a range
 // holds at most one of each.
 __host__ __device__ inline size_t paged_part_floats(int block_rows) { return (size_t)block_rows * (kCkv + 2); }
 __device__ __forceinline__ float* paged_part(const PagedArgs& a, int block_rows, int rb, int range, int which) {

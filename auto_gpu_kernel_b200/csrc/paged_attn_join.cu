@@ -27,8 +27,7 @@ paged_join_kernel(const PagedArgs a) {
   __shared__ float4 acc_sh[kSplit > 1 ? kSplit : 1][kGroup];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int b = (int)(blockIdx.x / a.rows), r = (int)(blockIdx.x % a.rows);
-  ptx::grid_dependency_wait();
-  ptx::launch_dependents();
+  // lengths are older than the attention kernel, which waits for its own predecessor before it lets this one start
   int lo, hi;
   long long before;
   const long long total = paged_scan<kThreads>(a.seq_lens, a.batch, a.max_pages, sums, lo, hi, before);
@@ -40,6 +39,8 @@ paged_join_kernel(const PagedArgs a) {
   const long long per = (total + a.grid_x - 1) / a.grid_x;
   const long long first = base_sh, last = first + paged_tiles(__ldg(a.seq_lens + b), a.max_pages) - 1;
   const int x0 = (int)(first / per), n_seg = (int)(last / per) - x0 + 1;
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
   if (n_seg == 1) return;               // the attention wrote this request itself
   const int rb = r / a.block_rows, br = r - rb * a.block_rows;
   const size_t stat = (size_t)a.block_rows * kCkv + br;
@@ -106,6 +107,85 @@ paged_join_kernel(const PagedArgs a) {
   if (blockIdx.y == 0 && tid == 0) a.lse[row] = sum == 0.f ? -INFINITY : mx + log2f(sum);
 }
 
+// The same for row blocks of 64, whose partial accumulators lie [column][row]: 64 threads have a row and eight columns
+// each, kSplit groups of them share the segments out, each with a running maximum of its own.
+constexpr int kJoinRows = 64, kJoinCols = 8;
+template <int kSplit>
+__global__ void __launch_bounds__(kSplit * kJoinRows)
+paged_join_columns_kernel(const PagedArgs a) {
+  constexpr int kThreads = kSplit * kJoinRows;
+  __shared__ long long sums[kThreads / 32];
+  __shared__ long long base_sh;
+  __shared__ float acc_sh[kSplit][kJoinCols + 2][kJoinRows];
+  const int tid = threadIdx.x, row = tid % kJoinRows, grp = tid / kJoinRows;
+  const int blocks = (a.rows + kJoinRows - 1) / kJoinRows;
+  const int b = (int)(blockIdx.x / blocks), rb = (int)(blockIdx.x % blocks);
+  // lengths are older than the attention kernel, which waits for its own predecessor before it lets this one start
+  int lo, hi;
+  long long before;
+  const long long total = paged_scan<kThreads>(a.seq_lens, a.batch, a.max_pages, sums, lo, hi, before);
+  for (int k = lo; k < hi; ++k) {
+    if (k == b) base_sh = before;
+    before += paged_tiles(__ldg(a.seq_lens + k), a.max_pages);
+  }
+  __syncthreads();
+  const long long per = (total + a.grid_x - 1) / a.grid_x;
+  const long long first = base_sh, last = first + paged_tiles(__ldg(a.seq_lens + b), a.max_pages) - 1;
+  const int x0 = (int)(first / per), n_seg = (int)(last / per) - x0 + 1;
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  if (n_seg == 1) return;
+  const int col = blockIdx.y * kJoinCols;
+  float m = -INFINITY, l = 0.f, v[kJoinCols];
+#pragma unroll
+  for (int k = 0; k < kJoinCols; ++k) v[k] = 0.f;
+  // one more partial result (m2, l2, u) into (m, l, v); an empty one has m2 = -inf and l2 = 0, one of NaNs l2 = NaN
+  auto add = [&](float m2, float l2, const float (&u)[kJoinCols]) {
+    const float mx = fmaxf(m, m2);
+    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - mx);
+    const float f = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : exp2f(m2 - mx);
+    m = mx;
+    l = l * c + l2 * f;
+#pragma unroll
+    for (int k = 0; k < kJoinCols; ++k) v[k] = v[k] * c + u[k] * f;
+  };
+#pragma unroll 4
+  for (int s = grp; s < n_seg; s += kSplit) {
+    const float* p = paged_part(a, kJoinRows, rb, x0 + s, s == 0 ? 1 : 0);
+    float u[kJoinCols];
+#pragma unroll
+    for (int k = 0; k < kJoinCols; ++k) u[k] = __ldcg(p + (size_t)(col + k) * kJoinRows + row);
+    const float m2 = __ldcg(p + (size_t)kJoinRows * kCkv + row), l2 = __ldcg(p + (size_t)kJoinRows * (kCkv + 1) + row);
+    add(m2, l2, u);
+  }
+  if (kSplit > 1) {
+#pragma unroll
+    for (int k = 0; k < kJoinCols; ++k) acc_sh[grp][k][row] = v[k];
+    acc_sh[grp][kJoinCols][row] = m;
+    acc_sh[grp][kJoinCols + 1][row] = l;
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll 1
+    for (int s = 1; s < kSplit; ++s) {
+      float u[kJoinCols];
+#pragma unroll
+      for (int k = 0; k < kJoinCols; ++k) u[k] = acc_sh[s][k][row];
+      add(acc_sh[s][kJoinCols][row], acc_sh[s][kJoinCols + 1][row], u);
+    }
+  }
+  const int r = rb * kJoinRows + row;
+  if (r >= a.rows) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t h[kJoinCols / 2];
+#pragma unroll
+  for (int k = 0; k < kJoinCols / 2; ++k) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k] * inv, v[2 * k + 1] * inv);
+    h[k] = *reinterpret_cast<const uint32_t*>(&t);
+  }
+  *reinterpret_cast<uint4*>(a.out + ((size_t)b * a.rows + r) * kCkv + col) = make_uint4(h[0], h[1], h[2], h[3]);
+  if (blockIdx.y == 0) a.lse[(size_t)b * a.rows + r] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
 // One thread per cached token, 256 tokens of one request per CTA; a row's 64 logits of a page are one coalesced
 // 256-byte read, and the rows are added in ascending order.
 constexpr int kWeighThreads = 256;
@@ -157,6 +237,12 @@ cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, cudaS
 
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t stream) {
   const unsigned rows = (unsigned)a.batch * (unsigned)a.rows;
+  if (a.block_rows == kJoinRows) {
+    const unsigned n = (unsigned)a.batch * (unsigned)((a.rows + kJoinRows - 1) / kJoinRows);
+    // segments per request: about ranges / (requests x row blocks)
+    if (n <= 4) return launch_after(paged_join_columns_kernel<16>, dim3(n, kCkv / kJoinCols), 16 * kJoinRows, stream, a);
+    return launch_after(paged_join_columns_kernel<4>, dim3(n, kCkv / kJoinCols), 4 * kJoinRows, stream, a);
+  }
   if (rows <= 160) return launch_after(paged_join_kernel<16, 128>, dim3(rows, 4), 512, stream, a);
   return launch_after(paged_join_kernel<1, 512>, dim3(rows), 128, stream, a);
 }

@@ -435,10 +435,6 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
 
 }  // namespace
 
-// Rows of a block: 16 query rows where a request has no more, else 32 (both products of a page then serve two row
-// groups, and the cache is read half as often).
-int paged_block_rows(int rows) { return rows <= 16 ? 16 : 32; }
-
 template <int MT, bool kLogits>
 static cudaError_t launch_one(const PagedArgs& a, const CUtensorMap& mc, const CUtensorMap& mk, int blocks, cudaStream_t stream) {
   static std::atomic<uint64_t> opted{0};
@@ -464,8 +460,8 @@ cudaError_t launch_paged_attn_mma(const PagedArgs& a, const void* ckv, const voi
   if (!make_tmap_2d_sw128(&mc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ckv, kCkv, slots, 64, kPage) ||
       !make_tmap_2d_sw128(&mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kpe, kKpe, slots, 64, kPage))
     return cudaErrorInvalidValue;
-  const int br = paged_block_rows(a.rows), blocks = (a.rows + br - 1) / br;
-  if (br == 16)
+  const int blocks = (a.rows + a.block_rows - 1) / a.block_rows;
+  if (a.block_rows == 16)
     return a.logits ? launch_one<1, true>(a, mc, mk, blocks, stream) : launch_one<1, false>(a, mc, mk, blocks, stream);
   return a.logits ? launch_one<2, true>(a, mc, mk, blocks, stream) : launch_one<2, false>(a, mc, mk, blocks, stream);
 }

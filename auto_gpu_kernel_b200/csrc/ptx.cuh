@@ -33,6 +33,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// The same question without the suspension that try_wait may take when the answer is no: for one thread that looks
+// at several barriers in turn.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ uint64_t global_timer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -189,6 +202,25 @@ __device__ __forceinline__ void mma_bf16_split(uint32_t d_tmem, uint32_t a_lo, u
       : "memory");
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+// kind::f16 (bf16 inputs) for a whole converged warp, issued by the lane whose `elected` is set.  In a branch of one
+// lane every operand has to be moved to a uniform register first (55-160 cycles per instruction measured); here
+// the descriptors are computed there, and M = 64, N = 64 issues every 36 cycles, M = 128, N = 64 every 49.
+__device__ __forceinline__ void mma_bf16_warp(uint32_t elected, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                              uint32_t idesc_v, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc_v), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+
 // TMEM -> registers: this warp's 32 lanes x 32 consecutive fp32 columns starting at taddr.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -213,7 +245,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-
+// TMEM -> registers, 16 lanes x 32 fp32 columns in the fragment order of mma.m16n8: r[4 n + e] is column
+// 8 n + 2 (lane % 4) + (e & 1) of lane lane / 4 + 8 (e >> 1) of the sixteen.
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 
 // ---------------------------------------------------------------- cp.async (LDGSTS) + named barriers
 // 16-byte global -> shared copy; src_bytes = 0 writes 16 zero bytes without reading `src`.
@@ -244,6 +287,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
         "r"(r[15])
       : "memory");
+}
+
+// 2^x, two steps off at most; results below 2^-126 become zero.
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Programmatic dependent launch: a kernel launched with the programmatic-stream-serialization
