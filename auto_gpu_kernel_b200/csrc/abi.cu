@@ -487,6 +487,7 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
   a.tokens = tokens_per_request;
   a.block_rows = dsa::paged_block_rows(rows);
   a.grid_x = paged_ranges(batch, paged_blocks(rows), max_pages);
+  a.switch_cost = dsa::paged_switch_cost(rows);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = a.block_rows == 64 ? dsa::launch_paged_attn_tc(a, ckv, kpe, s) : dsa::launch_paged_attn_mma(a, ckv, kpe, s);
   if (e == cudaSuccess && a.grid_x > 1) e = dsa::launch_paged_join(a, s);

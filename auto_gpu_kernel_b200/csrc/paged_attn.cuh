@@ -2,11 +2,14 @@
 // the places of the partial results.
 //
 // A request of `len` cached tokens is max(1, ceil(len / 64)) tiles of one page each (the one tile of an empty
-// request holds nothing and writes its zero output).  The tiles of all requests, one after the other, are cut into
-// equal ranges, one per CTA of a row block; where a request is cut, every CTA that has a part of it (a "segment")
+// request holds nothing and writes its zero output).  The tiles of all requests, one after the other and each request
+// with `switch_cost` units of nothing in front, are cut into equal ranges, one per CTA of a row block: taking up a
+// request (its q, its output) costs about that many tiles, and a CTA with ten short requests would otherwise end
+// long after one that is inside a long one.  Where a request is cut, every CTA that has a part of it (a "segment")
 // leaves a partial result.  Lengths live on the device, so every CTA works the split out for itself.
 #pragma once
 
+#include <cstdlib>
 #include "common.cuh"
 
 namespace dsa {
@@ -28,6 +31,7 @@ struct PagedArgs {
   int heads, tokens;
   int block_rows;   // query rows that a CTA takes at once (a row block)
   int grid_x;       // ranges the tiles are cut into
+  int switch_cost;  // what taking up a request costs, in tiles
 };
 
 constexpr int kPagedMaxRanges = 512;
@@ -35,6 +39,7 @@ constexpr int kPagedMaxRanges = 512;
 // Query rows that a CTA takes at once, from the rows of a request: 16 or 32 by warp-level products (one or two row
 // groups per page), 64 by tcgen05.
 inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+inline int paged_switch_cost(int rows) { const char* e = getenv("SWC"); return e ? atoi(e) : (rows <= 32 ? 2 : 4); }
 
 __host__ __device__ inline int paged_len(int len, int max_pages) {
   const int64_t most = (int64_t)max_pages * kPage;
@@ -56,13 +61,12 @@ __device__ __forceinline__ float* paged_part(const PagedArgs& a, int block_rows,
 // Sum of all requests' tiles, and the tiles in front of this thread's share of the requests (requests
 // [lo, hi) of equal contiguous shares).  By all threads of the CTA; `sums` has one entry per warp.
 template <int kThreads>
-__device__ __forceinline__ long long paged_scan(const int32_t* seq_lens, int batch, int max_pages, long long* sums,
-                                                int& lo, int& hi, long long& before) {
-  const int share = (batch + kThreads - 1) / kThreads;
-  lo = min((int)threadIdx.x * share, batch);
-  hi = min(lo + share, batch);
+__device__ __forceinline__ long long paged_scan(const PagedArgs& a, long long* sums, int& lo, int& hi, long long& before) {
+  const int share = (a.batch + kThreads - 1) / kThreads;
+  lo = min((int)threadIdx.x * share, a.batch);
+  hi = min(lo + share, a.batch);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += paged_tiles(__ldg(seq_lens + b), max_pages);
+  for (int b = lo; b < hi; ++b) mine += paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
   long long upto = mine;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
@@ -80,6 +84,66 @@ __device__ __forceinline__ long long paged_scan(const int32_t* seq_lens, int bat
   }
   before = front + upto - mine;
   return total;
+}
+
+// Units of a range, and the unit that request b's tiles begin at when `tiles` tiles lie in front of it.
+__device__ __forceinline__ long long paged_units(const PagedArgs& a, long long total) {
+  return (total + (long long)a.batch * a.switch_cost + a.grid_x - 1) / a.grid_x;
+}
+__device__ __forceinline__ long long paged_first_unit(const PagedArgs& a, int b, long long tiles) {
+  return tiles + (long long)(b + 1) * a.switch_cost;
+}
+
+// The tiles of range `range`: from tile start_j of request start_b on, end - begin in number (tiles counted over
+// all requests).  By all threads of the CTA; a __syncthreads must follow before the words are read.
+struct PagedRange {
+  long long begin, end;
+  int start_b, start_j;
+};
+template <int kThreads>
+__device__ __forceinline__ void paged_find_range(const PagedArgs& a, int range, long long* sums, PagedRange* out) {
+  int lo, hi;
+  long long before;
+  const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
+  const long long per = paged_units(a, total), v0 = range * per, v1 = v0 + per;
+  if (threadIdx.x == 0) {
+    // (a range behind the last unit has no tiles)
+    if (v0 >= total + (long long)a.batch * a.switch_cost) out->begin = total;
+    if (v1 >= total + (long long)a.batch * a.switch_cost) out->end = total;
+  }
+  for (int b = lo; b < hi; ++b) {
+    const int k = paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
+    const long long first = paged_first_unit(a, b, before), begin = first - a.switch_cost, end = first + k;
+    if (v0 >= begin && v0 < end) {
+      const int j = v0 > first ? (int)(v0 - first) : 0;
+      out->begin = before + j;
+      out->start_b = b;
+      out->start_j = j;
+    }
+    if (v1 >= begin && v1 < end) out->end = before + (v1 > first ? v1 - first : 0);
+    before += k;
+  }
+}
+
+// The segments of request b: ranges first .. first + count - 1.  By all threads of the CTA, the same contract.
+struct PagedSegments {
+  int first, count;
+};
+template <int kThreads>
+__device__ __forceinline__ void paged_find_segments(const PagedArgs& a, int b, long long* sums, PagedSegments* out) {
+  int lo, hi;
+  long long before;
+  const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
+  const long long per = paged_units(a, total);
+  for (int k = lo; k < hi && k <= b; ++k) {
+    const int tiles = paged_tiles(__ldg(a.seq_lens + k), a.max_pages);
+    if (k == b) {
+      const long long first = paged_first_unit(a, b, before);
+      out->first = (int)(first / per);
+      out->count = (int)((first + tiles - 1) / per) - out->first + 1;
+    }
+    before += tiles;
+  }
 }
 
 }  // namespace dsa

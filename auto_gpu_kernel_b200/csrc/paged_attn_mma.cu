@@ -12,8 +12,8 @@
 // ckv column blocks and kpe) with the 128-byte swizzle, which keeps both ldmatrix patterns free of bank conflicts;
 // nine lanes of warp 0 issue a page's boxes two pages ahead, into the stage that the page before the current one has
 // just left, and look the page ids up 32 at a time, one batch ahead.
-//   S = Q.K^T   warp w has the 16-row group w % MT of the block and 8 MT of the page's tokens; q stays in registers
-//               as 36 A fragments;
+//   S = Q.K^T   warp w has the 16-row group w % MT of the block and 8 MT of the page's tokens; q_nope stays in
+//               registers as 32 A fragments, q_pe in shared memory (all 36 left the loop no registers to schedule in);
 //   softmax     base 2, the running maximum refreshed (and O rescaled) only when a logit exceeds it by more than 2^8;
 //               P is rounded to bf16 for the second product, as the cache that it multiplies is bf16; sums are taken
 //               of the fp32 values;
@@ -34,7 +34,7 @@ constexpr int kPaStages = 3;
 constexpr int kPaBlockBytes = kPage * 128;           // 8192
 constexpr int kPaStageBytes = 9 * kPaBlockBytes;     // 73728
 constexpr int kPaThreads = 256;
-constexpr int kPaQPitch = 1168;                      // 1152-byte q rows, padded against bank conflicts
+constexpr int kPaQPitch = 1040;                      // 1024-byte q_nope rows, padded against bank conflicts
 constexpr float kPaRescaleGap = 8.f;
 
 struct PaTile {
@@ -45,13 +45,12 @@ struct PaShared {
   PaTile tile[kPaStages];
   float red[8 * kHeads];        // [token group][block row]
   long long sums[kPaThreads / 32];
-  long long start_base;
-  int start_b;
+  PagedRange range;
 };
 
 template <int MT>
 constexpr size_t pa_dyn_bytes() {
-  return 1024 + kPaStages * kPaStageBytes + 16 * MT * 128 + sizeof(PaShared);
+  return 1024 + kPaStages * kPaStageBytes + 2 * 16 * MT * 128 + sizeof(PaShared);
 }
 
 template <int MT, bool kLogits>
@@ -67,7 +66,8 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
   unsigned char* kv_ptr = dyn_raw + pad;
   const uint32_t p_addr = kv_addr + kPaStages * kPaStageBytes;
   unsigned char* p_ptr = kv_ptr + kPaStages * kPaStageBytes;
-  PaShared& sh = *reinterpret_cast<PaShared*>(p_ptr + kRows * 128);
+  const uint32_t qpe_addr = p_addr + kRows * 128;
+  PaShared& sh = *reinterpret_cast<PaShared*>(p_ptr + 2 * kRows * 128);
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -84,27 +84,14 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
   ptx::launch_dependents();
 
   // ---------------- this CTA's range of tiles --------------------------------------------------------
-  int lo, hi;
-  long long before;
-  const long long total = paged_scan<kPaThreads>(a.seq_lens, a.batch, a.max_pages, sh.sums, lo, hi, before);
-  const long long per = (total + a.grid_x - 1) / a.grid_x;
-  const long long w0 = (long long)range * per;
-  const long long w1 = w0 + per < total ? w0 + per : total;
-  const int n = w0 < w1 ? (int)(w1 - w0) : 0;
-  if (n == 0) return;
-  for (int b = lo; b < hi; ++b) {
-    const int k = paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
-    if (w0 >= before && w0 < before + k) {
-      sh.start_b = b;
-      sh.start_base = before;
-    }
-    before += k;
-  }
+  paged_find_range<kPaThreads>(a, range, sh.sums, &sh.range);
   __syncthreads();
+  const int n = (int)(sh.range.end - sh.range.begin);
+  if (n <= 0) return;
 
   // ---------------- tile issue (warp 0) --------------------------------------------------------------
   int issued = 0;
-  int ib = sh.start_b, ij = (int)(w0 - sh.start_base), ilen = 0, itiles = 0, cbase = ij;
+  int ib = sh.range.start_b, ij = sh.range.start_j, ilen = 0, itiles = 0, cbase = ij;
   int cur = -1, nb = 0, nc = 0, nxt = -1, nlen = 0;
   auto lookup = [&](int b, int c) {      // page ids of tiles c .. c+31 of request b, one per lane
     return b < a.batch && c + lane < a.max_pages ? __ldg(a.block_table + (int64_t)b * a.table_stride + c + lane) : -1;
@@ -162,16 +149,21 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       const int r = rb * kRows + h;
       const size_t row = (size_t)b * a.rows + (r < a.rows ? r : 0);
       const __nv_bfloat16* src = jj < 64 ? a.q_nope + row * kCkv + jj * 8 : a.q_pe + row * kKpe + (jj - 64) * 8;
-      ptx::cp_async16(qs + h * kPaQPitch + jj * 16, src, r < a.rows ? 16 : 0);
+      const uint32_t dst = jj < 64 ? qs + h * kPaQPitch + jj * 16 : qpe_addr + h * 128 + (((jj - 64) ^ (h & 7)) << 4);
+      ptx::cp_async16(dst, src, r < a.rows ? 16 : 0);
     }
     cp_async_commit();
   };
-  stage_q(sh.start_b, kv_addr + 2 * kPaStageBytes);   // tile 2 gets the stage once q is in registers
+  stage_q(sh.range.start_b, kv_addr + 2 * kPaStageBytes);   // tile 2 gets the stage once q is in registers
   if (w == 0) {
     issue_tile();
     issue_tile();
   }
 
+  // where the logits of a tile go (only where they are wanted)
+  auto tile_logits = [&](const PaTile& t) {
+    return a.logits + (((size_t)t.b * a.max_pages + t.j) * gridDim.y + rb) * (size_t)(kRows * kPage);
+  };
   // token (of the request's new ones) of each row of this thread; rows behind the last see nothing
   int row_tok[MT][2];
 #pragma unroll
@@ -183,7 +175,7 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
     }
   }
 
-  uint32_t qa[36][4];           // A fragments of q: k-step ks covers columns 16 ks .. 16 ks + 15
+  uint32_t qa[32][4];           // A fragments of q_nope: k-step ks covers columns 16 ks .. 16 ks + 15
   float o[MT][8][4];            // O[rows 16m+g / +8][columns 64 w + 8 n + 2 t4, +1]
   float m_run[MT][2];           // running maxima of all rows of the block that this thread accumulates
   float l0 = 0.f, l1 = 0.f;     // row sums over this thread's tokens, rows of group mt
@@ -207,7 +199,7 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       __syncthreads();
       const uint32_t qrow = qs + (16 * mt + (lane & 7) + ((lane >> 3) & 1) * 8) * kPaQPitch + (lane >> 4) * 16;
 #pragma unroll
-      for (int ks = 0; ks < 36; ++ks) ldsm_x4(qrow + ks * 32, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
+      for (int ks = 0; ks < 32; ++ks) ldsm_x4(qrow + ks * 32, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         m_run[m][0] = m_run[m][1] = -INFINITY;
@@ -227,12 +219,11 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
     }
     if (w == 0) issue_tile();          // tile i+2 -> the stage tile i-1 used
     const int pos0 = tile.j * kPage;
-    float* lg = nullptr;
-    if (kLogits)
-      lg = a.logits + (((size_t)tile.b * a.max_pages + tile.j) * gridDim.y + rb) * (size_t)(kRows * kPage);
     if (!tile.live) {
-      if (kLogits && tile.len > 0)
+      if (kLogits && tile.len > 0) {
+        float* lg = tile_logits(tile);
         for (int c = tid; c < kRows * kPage; c += kPaThreads) lg[c] = -INFINITY;
+      }
     } else {
       const uint32_t sa = kv_addr + s * kPaStageBytes;
       const int filled = tile.len - pos0;
@@ -260,8 +251,19 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
             uint32_t r0, r1, r2, r3;
             ldsm_x4(brow + kb * kPaBlockBytes + (((kk * 4 + quad) ^ rx) << 4), r0, r1, r2, r3);
             const int c = MT == 1 ? 2 * kk : 2 * t;
-            hmma_16816(acc[c], qa[kb * 4 + 2 * kk], r0, r1);
-            hmma_16816(acc[c + 1], qa[kb * 4 + 2 * kk + 1], r2, r3);
+            if (kb < 8) {
+              hmma_16816(acc[c], qa[kb * 4 + 2 * kk], r0, r1);
+              hmma_16816(acc[c + 1], qa[kb * 4 + 2 * kk + 1], r2, r3);
+            } else {                     // q_pe
+              const int qr = 16 * mt + (lane & 7) + ((lane >> 3) & 1) * 8;
+              uint32_t qp[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                ldsm_x4(qpe_addr + qr * 128 + (((4 * kk + 2 * h + (lane >> 4)) ^ (qr & 7)) << 4), qp[h][0], qp[h][1], qp[h][2],
+                        qp[h][3]);
+              hmma_16816(acc[c], qp[0], r0, r1);
+              hmma_16816(acc[c + 1], qp[1], r2, r3);
+            }
           }
         }
       }
@@ -279,10 +281,6 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
         const int r0 = 16 * mt + g;
         pw[t][0] = reinterpret_cast<uint32_t*>(p_ptr + r0 * 128 + ((chunk ^ (g & 7)) << 4) + t4 * 4);
         pw[t][1] = reinterpret_cast<uint32_t*>(p_ptr + (r0 + 8) * 128 + ((chunk ^ (g & 7)) << 4) + t4 * 4);
-        if (kLogits) {
-          *reinterpret_cast<float2*>(lg + r0 * kPage + 8 * chunk + 2 * t4) = make_float2(x[t][0], x[t][1]);
-          *reinterpret_cast<float2*>(lg + (r0 + 8) * kPage + 8 * chunk + 2 * t4) = make_float2(x[t][2], x[t][3]);
-        }
       }
       float v0 = fmaxf(x[0][0], x[0][1]), v1 = fmaxf(x[0][2], x[0][3]);
 #pragma unroll
@@ -350,6 +348,14 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       for (int t = 0; t < MT; ++t) {
         l0 += p[t][0] + p[t][1];
         l1 += p[t][2] + p[t][3];
+      }
+      if (kLogits) {                    // behind the barrier that the other warps wait at
+        float* lg = tile_logits(tile) + (16 * mt + g) * kPage + 8 * MT * tg + 2 * t4;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          *reinterpret_cast<float2*>(lg + 8 * t) = make_float2(x[t][0], x[t][1]);
+          *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * t) = make_float2(x[t][2], x[t][3]);
+        }
       }
       // ---- O += P . V for columns 64w .. 64w+63 (column block w of the tile) ---------------------
       {

@@ -49,8 +49,7 @@ struct TcShared {
   float corr[kTcRows], inv[kTcRows];   // of each row: what O^T is multiplied by in a refresh, and at the end
   float half[2][kTcRows];              // maxima, at the end sums, over the token halves
   long long sums[kTcThreads / 32];
-  long long start_base;
-  int start_b;
+  PagedRange range;
   alignas(16) int word[4][8];          // what the softmax warps tell each other at a barrier: 1 = refresh, 2 = a wait ran out
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -98,26 +97,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
   }
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  int lo, hi;
-  long long before;
-  const long long total = paged_scan<kTcThreads>(a.seq_lens, a.batch, a.max_pages, sh.sums, lo, hi, before);
-  const long long per = (total + a.grid_x - 1) / a.grid_x;
-  const long long w0 = (long long)range * per;
-  const long long w1 = w0 + per < total ? w0 + per : total;
-  const int n = w0 < w1 ? (int)(w1 - w0) : 0;
-  if (n > 0) {
-    for (int b = lo; b < hi; ++b) {
-      const int k = paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
-      if (w0 >= before && w0 < before + k) {
-        sh.start_b = b;
-        sh.start_base = before;
-      }
-      before += k;
-    }
-  }
+  paged_find_range<kTcThreads>(a, range, sh.sums, &sh.range);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
+  const int n = (int)(sh.range.end - sh.range.begin);
   const uint32_t tmem = sh.tmem_base;
 
   if (n > 0 && warp < 8) {
@@ -470,7 +454,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
     __syncwarp();
   } else if (n > 0) {
     // ============================ TMA producer ============================
-    int ib = sh.start_b, ij = (int)(w0 - sh.start_base), cbase = ij, qb = -1, nq = 0;
+    int ib = sh.range.start_b, ij = sh.range.start_j, cbase = ij, qb = -1, nq = 0;
     int ilen = paged_len(__ldg(a.seq_lens + ib), a.max_pages), itiles = paged_tiles(ilen, a.max_pages);
     int cur, nb = 0, nc = 0, nxt = -1, nlen = 0;
     auto lookup = [&](int b, int c) {
