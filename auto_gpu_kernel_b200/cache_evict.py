@@ -10,16 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, workspace
-from .paged_attention import PAGE, check_caches, check_tables
-
-
-def _rows(name, t, batch, width, dtype, device):
-    if t.dim() != 2 or t.shape[0] != batch or t.shape[1] < width or t.dtype != dtype \
-            or (t.shape[1] > 1 and t.stride(1) != 1) or (batch > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"cache eviction: {name} must be [{batch},>= {width}] {dtype} with dense rows of their own")
-    if t.device != device:
-        raise RuntimeError(f"cache eviction: {name} must be on {device}")
-    return t.data_ptr(), max(t.stride(0), t.shape[1])
+from .paged_attention import PAGE, caches_ok, refuse_caches, refuse_tables, rows_of, tables_ok
 
 
 def kernel(token_weights, seq_lens, block_table, new_block_table, budget, ckv_cache, kpe_cache, k_index_cache_fp8,
@@ -36,34 +27,40 @@ def kernel(token_weights, seq_lens, block_table, new_block_table, budget, ckv_ca
     A page of new_block_table must not be one that a request of this call still reads from, unless every kept
     token on it keeps its place (a request within the budget may pass its old row: nothing moves then), and must
     not stand in it twice: such moves race."""
+    what = "cache eviction"
     if not token_weights.is_cuda:
-        raise RuntimeError("cache eviction: CUDA tensors required (this operator has no CPU path)")
-    dev = token_weights.device
+        raise RuntimeError(f"{what}: CUDA tensors required (this operator has no CPU path)")
+    index = token_weights.get_device()
     budget = int(budget)
     if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
-        raise ValueError("cache eviction: budget >= 1 and 0 <= keep_first + keep_last <= budget")
-    batch, max_pages = check_tables("cache eviction", seq_lens, block_table, dev)
-    pages = check_caches("cache eviction", ckv_cache, kpe_cache, dev)
-    new_batch, new_pages = check_tables("cache eviction (new_block_table)", seq_lens, new_block_table, dev)
+        raise ValueError(f"{what}: budget >= 1 and 0 <= keep_first + keep_last <= budget")
+    if not tables_ok(seq_lens, block_table, index):
+        refuse_tables(what, seq_lens, block_table, index)
+    if not tables_ok(seq_lens, new_block_table, index):
+        refuse_tables(f"{what} (new_block_table)", seq_lens, new_block_table, index)
+    if not caches_ok(ckv_cache, kpe_cache, index):
+        refuse_caches(what, ckv_cache, kpe_cache, index)
+    batch, max_pages = block_table.shape
+    pages, new_pages = ckv_cache.shape[0], new_block_table.shape[1]
     if new_pages * PAGE < min(budget, max_pages * PAGE):
-        raise ValueError(f"cache eviction: new_block_table has room for {new_pages * PAGE} tokens of a budget of {budget}")
-    index = 0
+        raise ValueError(f"{what}: new_block_table has room for {new_pages * PAGE} tokens of a budget of {budget}")
+    keys = 0
     if k_index_cache_fp8 is not None:
         if k_index_cache_fp8.shape != (pages, PAGE, 1, 132) or k_index_cache_fp8.element_size() != 1 \
                 or not k_index_cache_fp8.is_contiguous():
-            raise ValueError("cache eviction: k_index_cache_fp8 must be a contiguous [P,64,1,132] int8 tensor with as many "
-                             "pages as ckv_cache")
-        if k_index_cache_fp8.device != dev:
-            raise RuntimeError(f"cache eviction: k_index_cache_fp8 must be on {dev}")
-        index = k_index_cache_fp8.data_ptr()
-    if new_seq_lens.shape != (batch,) or new_seq_lens.dtype != torch.int32 or not new_seq_lens.is_contiguous() \
-            or new_seq_lens.device != dev:
-        raise ValueError(f"cache eviction: new_seq_lens must be a contiguous [B] int32 tensor on {dev}")
-    w, w_stride = _rows("token_weights", token_weights, batch, max_pages * PAGE, torch.float32, dev)
-    nw, nw_stride = _rows("new_token_weights", new_token_weights, batch, budget, torch.float32, dev)
-    kept, kept_stride = _rows("kept_positions", kept_positions, batch, budget, torch.int32, dev)
+            raise ValueError(f"{what}: k_index_cache_fp8 must be a contiguous [P,64,1,132] int8 tensor with as many pages "
+                             "as ckv_cache")
+        if k_index_cache_fp8.get_device() != index:
+            raise RuntimeError(f"{what}: k_index_cache_fp8 must be on cuda:{index}")
+        keys = k_index_cache_fp8.data_ptr()
+    if new_seq_lens.dim() != 1 or new_seq_lens.shape[0] != batch or new_seq_lens.dtype is not torch.int32 \
+            or not new_seq_lens.is_contiguous() or new_seq_lens.get_device() != index:
+        raise ValueError(f"{what}: new_seq_lens must be a contiguous [B] int32 tensor on cuda:{index}")
+    w, w_stride = rows_of(what, "token_weights", token_weights, batch, max_pages * PAGE, torch.float32, index)
+    nw, nw_stride = rows_of(what, "new_token_weights", new_token_weights, batch, budget, torch.float32, index)
+    kept, kept_stride = rows_of(what, "kept_positions", kept_positions, batch, budget, torch.int32, index)
     if workspace.overlap(token_weights, new_token_weights) or workspace.overlap(seq_lens, new_seq_lens):
-        raise ValueError("cache eviction: the outputs must not overlap the inputs")
+        raise ValueError(f"{what}: the outputs must not overlap the inputs")
     if batch == 0:
         return None
     if max_pages == 0:
@@ -72,13 +69,13 @@ def kernel(token_weights, seq_lens, block_table, new_block_table, budget, ckv_ca
         kept_positions[:, :budget].fill_(-1)
         return None
     lib = _lib.load()
-    with workspace.device_guard(dev):
-        rc = lib.dsa_cache_evict(
-            w, w_stride, seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), new_block_table.data_ptr(),
-            new_block_table.stride(0), ckv_cache.data_ptr(), kpe_cache.data_ptr(), index, new_seq_lens.data_ptr(), nw,
-            nw_stride, kept, kept_stride, batch, max_pages, new_pages, pages, budget, int(keep_first), int(keep_last),
-            workspace.status_word(dev).data_ptr(), workspace.stream_handle(dev))
-    _lib.check(rc, "dsa_cache_evict")
+    rc = workspace.call_on(
+        index, lib.dsa_cache_evict, w, w_stride, seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        new_block_table.data_ptr(), new_block_table.stride(0), ckv_cache.data_ptr(), kpe_cache.data_ptr(), keys,
+        new_seq_lens.data_ptr(), nw, nw_stride, kept, kept_stride, batch, max_pages, new_pages, pages, budget,
+        int(keep_first), int(keep_last))
+    if rc:
+        _lib.check(rc, "dsa_cache_evict")
     return None
 
 
@@ -86,13 +83,13 @@ def run(token_weights, seq_lens, block_table, new_block_table, budget, ckv_cache
         keep_first=0, keep_last=0, new_seq_lens=None, new_token_weights=None, kept_positions=None):
     """Value-returning form: allocates the outputs that are not passed; returns (new_seq_lens, new_token_weights,
     kept_positions)."""
-    batch, dev = seq_lens.shape[0], seq_lens.device
+    batch, width = seq_lens.shape[0], max(int(budget), 0)
     if new_seq_lens is None:
-        new_seq_lens = torch.empty(batch, dtype=torch.int32, device=dev)
+        new_seq_lens = seq_lens.new_empty((batch,))
     if new_token_weights is None:
-        new_token_weights = torch.empty(batch, budget, dtype=torch.float32, device=dev)
+        new_token_weights = token_weights.new_empty((batch, width))
     if kept_positions is None:
-        kept_positions = torch.empty(batch, budget, dtype=torch.int32, device=dev)
+        kept_positions = seq_lens.new_empty((batch, width))
     kernel(token_weights, seq_lens, block_table, new_block_table, budget, ckv_cache, kpe_cache, k_index_cache_fp8,
            new_seq_lens, new_token_weights, kept_positions, keep_first, keep_last)
     return new_seq_lens, new_token_weights, kept_positions

@@ -4,19 +4,27 @@
 //             the lower position), in ascending order; every position where a request is within the budget
 //   token j of the request moves from position kept(b)[j] of its old pages to position j of its new pages.
 //
-// Two kernels.  The choice is a radix selection over the order-preserving 32-bit keys of the weights (11 + 11 + 10 bits),
-// then one sweep that writes the kept positions in order; a row is read four times, from L2 after the first.  The
-// move is bound by memory: 1152 B (+ 132 B of an index key and its scale) in and out per kept token.
+// Two kernels.  The choice is a radix selection over the order-preserving 32-bit keys of the weights (11 + 11 + 10 bits):
+// a cluster of CTAs per request, each with a slice of the row as keys in shared memory, adds its three histograms up
+// through distributed shared memory; then every thread counts what it keeps of a run of its own, one scan gives the
+// places, and the positions are written in order.  It is a chain of sweeps and barriers, so the cluster is as large as
+// the machine allows while a slice stays worth a sweep.  The move is bound by memory: 1152 B (+ 132 B of an index key and
+// its scale) in and out per kept token; the kept weights go along with it.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
 
 namespace dsa {
 
+namespace cg = cooperative_groups;
+
 namespace {
 
 constexpr int kEvThreads = 1024;
 constexpr int kEvBins = 2048;
+constexpr int kEvStaged = 40960;      // keys of a slice that fit in shared memory; longer slices are read again
 
 struct EvictArgs {
   const float* weights;
@@ -49,38 +57,44 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
 }
 
 // Sum of `v` over the threads in front of this one, and over all of them.
-__device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t* sums, uint32_t& total) {
+template <typename T>
+__device__ __forceinline__ T ev_scan(T v, T* sums, T& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint32_t upto = v;
+  T upto = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+    const T u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
   if (lane == 31) sums[w] = upto;
   __syncthreads();
   if (w == 0) {
-    uint32_t s = sums[lane];
+    T s = sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+      const T u = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += u;
     }
     sums[lane] = s;
   }
   __syncthreads();
   total = sums[31];
-  const uint32_t r = (w ? sums[w - 1] : 0u) + upto - v;
+  const T r = (w ? sums[w - 1] : T(0)) + upto - v;
   __syncthreads();
   return r;
 }
 
 __global__ void __launch_bounds__(kEvThreads)
 evict_choose_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[kEvBins];
+  extern __shared__ uint32_t keys[];
+  __shared__ uint32_t hist[2][kEvBins];
   __shared__ uint32_t sums[32];
+  __shared__ uint64_t sums64[32];
   __shared__ uint32_t pick[2];
-  const int b = blockIdx.x, tid = threadIdx.x;
+  __shared__ uint64_t slice_counts;         // of this CTA's slice: above the threshold, and (high half) equal to it
+  cg::cluster_group cluster = cg::this_cluster();
+  const int csize = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int b = blockIdx.x / csize, tid = threadIdx.x;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   const int n = ev_len(a, b);
@@ -88,43 +102,63 @@ evict_choose_kernel(const EvictArgs a) {
   float* nw = a.new_weights + (int64_t)b * a.new_weights_stride;
   int32_t* kept = a.kept + (int64_t)b * a.kept_stride;
   const int m = n < a.budget ? n : a.budget;
-  if (tid == 0) a.new_lens[b] = m;
-  for (int j = m + tid; j < a.budget; j += kEvThreads) {
+  const int t0 = rank * kEvThreads + tid, step = csize * kEvThreads;
+  if (t0 == 0) a.new_lens[b] = m;
+  for (int j = m + t0; j < a.budget; j += step) {
     kept[j] = -1;
     nw[j] = 0.f;
   }
   if (n <= a.budget) {
-    for (int j = tid; j < n; j += kEvThreads) {
-      kept[j] = j;
-      nw[j] = w[j];
-    }
+    for (int j = t0; j < n; j += step) kept[j] = j;
     return;
   }
   const int lo = a.keep_first, hi = n - a.keep_last;      // budget < n: the ends do not meet
   const uint32_t want = (uint32_t)(a.budget - a.keep_first - a.keep_last);
-  for (int j = tid; j < lo; j += kEvThreads) {
-    kept[j] = j;
-    nw[j] = w[j];
-  }
-  for (int j = hi + tid; j < n; j += kEvThreads) {
-    kept[a.budget - n + j] = j;
-    nw[a.budget - n + j] = w[j];
-  }
+  for (int j = t0; j < lo; j += step) kept[j] = j;
+  for (int j = hi + t0; j < n; j += step) kept[a.budget - n + j] = j;
   if (want == 0) return;
 
+  // this CTA's slice of the positions in question
+  const int per = (hi - lo + csize - 1) / csize;
+  const int s0 = min(lo + rank * per, hi), cnt = min(s0 + per, hi) - s0;
+  const bool staged = cnt <= kEvStaged;
   // ---- the want-th largest key of positions lo .. hi-1, eleven, eleven and ten bits at a time ----
   uint32_t prefix = 0, rest = want;      // keys that begin with `prefix` are still in question; `rest` of them are kept
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
+    uint32_t* h = hist[pass & 1];        // the other one may still be read by the cluster
+    for (int i = tid; i < kEvBins; i += kEvThreads) h[i] = 0;
     __syncthreads();
-    for (int j = lo + tid; j < hi; j += kEvThreads) {
-      const uint32_t k = ev_key(w[j]);
-      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1u);
+    for (int j = tid; j < cnt; j += 8 * kEvThreads) {
+      uint32_t k[8];
+      if (pass == 0 || !staged) {
+        float v[8];                      // eight loads in flight
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = j + e * kEvThreads < cnt ? __ldg(w + s0 + j + e * kEvThreads) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          k[e] = ev_key(v[e]);
+          if (staged && j + e * kEvThreads < cnt) keys[j + e * kEvThreads] = k[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = j + e * kEvThreads < cnt ? keys[j + e * kEvThreads] : 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j + e * kEvThreads < cnt && (pass == 0 || (k[e] >> (shift + bits)) == prefix))
+          atomicAdd(&h[(k[e] >> shift) & ((1u << bits) - 1u)], 1u);
     }
-    __syncthreads();
-    // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
-    const uint32_t c0 = hist[kEvBins - 1 - 2 * tid], c1 = hist[kEvBins - 2 - 2 * tid];
+    if (csize > 1) cluster.sync();
+    else __syncthreads();
+    // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, of all slices
+    uint32_t c0 = h[kEvBins - 1 - 2 * tid], c1 = h[kEvBins - 2 - 2 * tid];
+    for (int r = 0; r < csize; ++r) {
+      if (r == rank) continue;
+      const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(h, r) + kEvBins - 2 - 2 * tid);
+      c0 += v.y;
+      c1 += v.x;
+    }
     uint32_t all;
     const uint32_t above = ev_scan(c0 + c1, sums, all);
     if (above < rest && above + c0 >= rest) {
@@ -140,60 +174,58 @@ evict_choose_kernel(const EvictArgs a) {
     __syncthreads();
   }
   // ---- keys above `prefix` are kept, and the first `rest` that equal it ----
-  uint32_t out = (uint32_t)lo, equal = 0;
-  for (int j0 = lo; j0 < hi; j0 += 4 * kEvThreads) {
-    uint32_t k[4];
-    float v[4];
-    uint32_t mine = 0;                   // above in the low half, equal in the high half (4096 at most)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = j0 + 4 * tid + e;
-      v[e] = j < hi ? w[j] : 0.f;
-      k[e] = ev_key(v[e]);
-      if (j < hi) mine += k[e] > prefix ? 1u : k[e] == prefix ? 0x10000u : 0u;
-    }
-    uint32_t all;
-    const uint32_t front = ev_scan(mine, sums, all);
-    uint32_t gt = front & 0xffffu, eq = equal + (front >> 16);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = j0 + 4 * tid + e;
-      if (j < hi) {
-        const bool above = k[e] > prefix, same = k[e] == prefix;
-        if (above || (same && eq < rest)) {
-          const uint32_t at = out + gt + min(eq, rest) - min(equal, rest);
-          kept[at] = j;
-          nw[at] = v[e];
-        }
-        gt += above;
-        eq += same;
-      }
-    }
-    const uint32_t eq_all = equal + (all >> 16);
-    out += (all & 0xffffu) + min(eq_all, rest) - min(equal, rest);
-    equal = eq_all;
+  // thread t has the run [t * run, (t + 1) * run) of the slice; an odd run keeps the banks apart
+  const int run = ((cnt + kEvThreads - 1) / kEvThreads) | 1;
+  const int j0 = min(tid * run, cnt), j1 = min(j0 + run, cnt);
+  uint64_t mine = 0, all64;
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t k = staged ? keys[j] : ev_key(w[s0 + j]);
+    mine += k > prefix ? 1ull : k == prefix ? 1ull << 32 : 0ull;
   }
+  mine = ev_scan(mine, sums64, all64);
+  if (csize > 1) {
+    if (tid == 0) slice_counts = all64;
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) mine += *cluster.map_shared_rank(&slice_counts, r);
+  }
+  uint32_t gt = (uint32_t)mine, eq = (uint32_t)(mine >> 32);
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t k = staged ? keys[j] : ev_key(w[s0 + j]);
+    if (k > prefix || (k == prefix && eq < rest)) kept[(uint32_t)lo + gt + min(eq, rest)] = s0 + j;
+    gt += k > prefix;
+    eq += k == prefix;
+  }
+  if (csize > 1) cluster.sync();         // nobody leaves while its counts may be read
 }
 
-// One warp per kRows kept tokens, all loads of a round in front of its stores.
+// Clusters of this many CTAs can be resident at once (a cluster needs its SMs inside one GPC).
+int ev_cluster(int batch, int64_t longest, int sms) {
+  int c = 1;
+  // a slice of 2048 keys is two sweeps of a CTA; less is not worth the cluster's barriers
+  while (c < 8 && longest / (2 * c) >= 2048 && (int64_t)batch * 2 * c <= (c == 4 ? sms * 4 / 5 : sms * 9 / 10)) c *= 2;
+  return c;
+}
+
+// One warp per four kept tokens: their slots are looked up together, then one row after the other moves.  More rows in
+// flight per warp cost registers and with them warps, and were slower (32 x 8192 rows with index keys: one row at a time
+// 117 us = 5.7 TB/s, two 125, four 156, eight 191 us; one lookup for every row 126 us).
 constexpr int kMvThreads = 256;
 constexpr int kMvRows = 4;
 
 template <bool kIndex>
 __global__ void __launch_bounds__(kMvThreads)
 evict_move_kernel(const EvictArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int b = blockIdx.y;
+  const int lane = threadIdx.x & 31, b = blockIdx.y;
   const int j0 = (blockIdx.x * (kMvThreads / 32) + (threadIdx.x >> 5)) * kMvRows;
+  const int n = ev_len(a, b), m = n < a.budget ? n : a.budget;    // older than the choice, which waits for its predecessor
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int n = ev_len(a, b), m = n < a.budget ? n : a.budget;
   if (j0 >= m) return;
-  // lane r < kMvRows works out the slots of the warp's row r
-  int64_t src = -1, dst = -1;
+  int64_t src = -1, dst = -1;              // lane r: row r
   if (lane < kMvRows && j0 + lane < m) {
     const int j = j0 + lane;
     const int from = __ldcg(a.kept + (int64_t)b * a.kept_stride + j);
+    a.new_weights[(int64_t)b * a.new_weights_stride + j] = __ldg(a.weights + (int64_t)b * a.weights_stride + from);
     const int p = __ldg(a.table + (int64_t)b * a.table_stride + from / kPage);
     const int q = __ldg(a.new_table + (int64_t)b * a.new_table_stride + j / kPage);
     if (p < 0 || p >= a.num_pages || q < 0 || q >= a.num_pages) {
@@ -201,41 +233,33 @@ evict_move_kernel(const EvictArgs a) {
     } else {
       src = (int64_t)p * kPage + from % kPage;
       dst = (int64_t)q * kPage + j % kPage;
-      if (src == dst) src = -1;          // keeps its place
+      if (src == dst) src = -1;            // keeps its place
     }
   }
-  uint4 c0[kMvRows], c1[kMvRows], e[kMvRows];
-  uint32_t sc[kMvRows];
-  int64_t s[kMvRows], d[kMvRows];
-#pragma unroll
+#pragma unroll 1
   for (int r = 0; r < kMvRows; ++r) {
-    s[r] = __shfl_sync(0xffffffffu, src, r);
-    d[r] = __shfl_sync(0xffffffffu, dst, r);
-    if (s[r] < 0) continue;
-    const uint4* row = a.ckv + s[r] * (kCkv * 2 / 16);
-    c0[r] = row[lane];
-    c1[r] = row[lane + 32];
+    const int64_t s = __shfl_sync(0xffffffffu, src, r), d = __shfl_sync(0xffffffffu, dst, r);
+    if (s < 0) continue;
+    const uint4* from = a.ckv + s * (kCkv * 2 / 16);
+    uint4* to = a.ckv + d * (kCkv * 2 / 16);
+    const uint4 c0 = from[lane], c1 = from[lane + 32];
     // lanes 0-7: kpe row; lanes 8-15: index key; lane 16: its scale
-    if (lane < 8) e[r] = a.kpe[s[r] * 8 + lane];
+    uint4 e = make_uint4(0, 0, 0, 0);
+    if (lane < 8) e = a.kpe[s * 8 + lane];
     if (kIndex) {
-      const uint8_t* page = a.index + (s[r] / kPage) * kPageBytes;
-      const int pos = (int)(s[r] % kPage);
-      if (lane >= 8 && lane < 16) e[r] = *reinterpret_cast<const uint4*>(page + pos * kIdxDim + (lane - 8) * 16);
-      if (lane == 16) sc[r] = *reinterpret_cast<const uint32_t*>(page + kPageDataBytes + pos * 4);
+      const uint8_t* page = a.index + (s / kPage) * kPageBytes;
+      const int pos = (int)(s % kPage);
+      if (lane >= 8 && lane < 16) e = *reinterpret_cast<const uint4*>(page + pos * kIdxDim + (lane - 8) * 16);
+      if (lane == 16) e.x = *reinterpret_cast<const uint32_t*>(page + kPageDataBytes + pos * 4);
     }
-  }
-#pragma unroll
-  for (int r = 0; r < kMvRows; ++r) {
-    if (s[r] < 0) continue;
-    uint4* row = a.ckv + d[r] * (kCkv * 2 / 16);
-    row[lane] = c0[r];
-    row[lane + 32] = c1[r];
-    if (lane < 8) a.kpe[d[r] * 8 + lane] = e[r];
+    to[lane] = c0;
+    to[lane + 32] = c1;
+    if (lane < 8) a.kpe[d * 8 + lane] = e;
     if (kIndex) {
-      uint8_t* page = a.index + (d[r] / kPage) * kPageBytes;
-      const int pos = (int)(d[r] % kPage);
-      if (lane >= 8 && lane < 16) *reinterpret_cast<uint4*>(page + pos * kIdxDim + (lane - 8) * 16) = e[r];
-      if (lane == 16) *reinterpret_cast<uint32_t*>(page + kPageDataBytes + pos * 4) = sc[r];
+      uint8_t* page = a.index + (d / kPage) * kPageBytes;
+      const int pos = (int)(d % kPage);
+      if (lane >= 8 && lane < 16) *reinterpret_cast<uint4*>(page + pos * kIdxDim + (lane - 8) * 16) = e;
+      if (lane == 16) *reinterpret_cast<uint32_t*>(page + kPageDataBytes + pos * 4) = e.x;
     }
   }
 }
@@ -250,21 +274,35 @@ cudaError_t launch_cache_evict(const float* weights, int64_t weights_stride, con
   EvictArgs a = {weights, weights_stride, seq_lens, table, table_stride, new_table, new_table_stride, static_cast<uint4*>(ckv),
                  static_cast<uint4*>(kpe), static_cast<uint8_t*>(index), new_lens, new_weights, new_weights_stride, kept,
                  kept_stride, status, batch, max_pages, num_pages, budget, keep_first, keep_last};
+  const int64_t longest = (int64_t)max_pages * kPage;
+  const int csize = ev_cluster(batch, longest, sm_count());
+  const int64_t slice = (longest + csize - 1) / csize;
+  const size_t staged = (size_t)(slice < kEvStaged ? slice : kEvStaged) * sizeof(uint32_t);
+  static std::atomic<uint64_t> opted{0};
+  cudaError_t e = opt_in_dynamic_smem(reinterpret_cast<const void*>(evict_choose_kernel), kEvStaged * sizeof(uint32_t), opted);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)batch);
+  cfg.gridDim = dim3((unsigned)(batch * csize));
   cfg.blockDim = dim3(kEvThreads);
+  cfg.dynamicSmemBytes = staged;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)csize;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, evict_choose_kernel, a);
+  cfg.numAttrs = csize > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, evict_choose_kernel, a);
   if (e != cudaSuccess) return e;
-  const int64_t most = (int64_t)max_pages * kPage < budget ? (int64_t)max_pages * kPage : budget;
+  const int64_t most = longest < budget ? longest : budget;
   const int per = kMvThreads / 32 * kMvRows;
   cfg.gridDim = dim3((unsigned)((most + per - 1) / per), (unsigned)batch);
   cfg.blockDim = dim3(kMvThreads);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
   return index ? cudaLaunchKernelEx(&cfg, evict_move_kernel<true>, a) : cudaLaunchKernelEx(&cfg, evict_move_kernel<false>, a);
 }
 

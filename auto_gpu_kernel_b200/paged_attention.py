@@ -19,39 +19,76 @@ PAGE = 64
 MAX_HEADS = 128
 
 
-def check_tables(what, seq_lens, block_table, device):
-    """Checks shared by the operators that walk a block table; returns (batch, max_pages)."""
+def tables_ok(seq_lens, block_table, index):
+    """seq_lens [B] and block_table [B,max_pages], int32 on the device of this index, as every operator here takes them."""
+    return (block_table.dim() == 2 and block_table.dtype is torch.int32 and seq_lens.dtype is torch.int32
+            and seq_lens.dim() == 1 and seq_lens.shape[0] == block_table.shape[0] and seq_lens.is_contiguous()
+            and (block_table.stride(1) == 1 or block_table.shape[1] <= 1)
+            and seq_lens.get_device() == index and block_table.get_device() == index)
+
+
+def refuse_tables(what, seq_lens, block_table, index):
+    """Say what `tables_ok` found wrong."""
     if block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise ValueError(f"{what}: block_table must be [B,max_pages] int32")
-    batch, max_pages = block_table.shape
-    if seq_lens.shape != (batch,) or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+    if seq_lens.shape != block_table.shape[:1] or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
         raise ValueError(f"{what}: seq_lens must be a contiguous [B] int32 tensor")
-    if max_pages > 1 and block_table.stride(1) != 1:
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
         raise ValueError(f"{what}: block_table rows must be dense (stride(1) == 1)")
-    if seq_lens.device != device or block_table.device != device:
-        raise RuntimeError(f"{what}: seq_lens and block_table must be on {device}")
-    return batch, max_pages
+    raise RuntimeError(f"{what}: seq_lens and block_table must be on cuda:{index}")
 
 
-def check_caches(what, ckv_cache, kpe_cache, device):
-    """The two paged caches, [P,64,512] and [P,64,64] bf16; returns P."""
+def caches_ok(ckv_cache, kpe_cache, index):
+    """The two paged caches, contiguous [P,64,512] and [P,64,64] bf16."""
+    c, k = ckv_cache.shape, kpe_cache.shape
+    return (len(c) == 3 and c[1] == PAGE and c[2] == CKV and len(k) == 3 and k[0] == c[0] and k[1] == PAGE and k[2] == KPE
+            and ckv_cache.dtype is torch.bfloat16 and kpe_cache.dtype is torch.bfloat16 and ckv_cache.is_contiguous()
+            and kpe_cache.is_contiguous() and ckv_cache.get_device() == index and kpe_cache.get_device() == index)
+
+
+def refuse_caches(what, ckv_cache, kpe_cache, index):
+    """Say what `caches_ok` found wrong."""
     if ckv_cache.dim() != 3 or ckv_cache.shape[1:] != (PAGE, CKV) or ckv_cache.dtype != torch.bfloat16 \
             or not ckv_cache.is_contiguous():
         raise ValueError(f"{what}: ckv_cache must be a contiguous [P,64,512] bf16 tensor")
-    pages = ckv_cache.shape[0]
-    if kpe_cache.shape != (pages, PAGE, KPE) or kpe_cache.dtype != torch.bfloat16 or not kpe_cache.is_contiguous():
+    if kpe_cache.shape != (ckv_cache.shape[0], PAGE, KPE) or kpe_cache.dtype != torch.bfloat16 \
+            or not kpe_cache.is_contiguous():
         raise ValueError(f"{what}: kpe_cache must be a contiguous [P,64,64] bf16 tensor with as many pages as ckv_cache")
-    if ckv_cache.device != device or kpe_cache.device != device:
-        raise RuntimeError(f"{what}: the caches must be on {device}")
-    return pages
+    raise RuntimeError(f"{what}: the caches must be on cuda:{index}")
 
 
-def _check_weights(name, t, batch, width, device):
-    if t.dim() != 2 or t.shape[0] != batch or t.shape[1] < width or t.dtype != torch.float32 \
-            or (t.shape[1] > 1 and t.stride(1) != 1) or (batch > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"paged attention: {name} must be [B,>= 64*max_pages] float32 with dense rows of their own")
-    if t.device != device:
-        raise RuntimeError(f"paged attention: {name} must be on {device}")
+def rows_of(what, name, t, batch, width, dtype, index):
+    """(address, row stride) of a [batch,>= width] tensor with dense rows of their own."""
+    if t.dim() != 2 or t.dtype is not dtype or t.shape[0] != batch or t.shape[1] < width \
+            or (t.stride(1) != 1 and t.shape[1] > 1) or (batch > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{what}: {name} must be [{batch},>= {width}] {dtype} with dense rows of their own")
+    if t.get_device() != index:
+        raise RuntimeError(f"{what}: {name} must be on cuda:{index}")
+    return t.data_ptr(), max(t.stride(0), t.shape[1])
+
+
+def _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, lse):
+    what = "paged attention"
+    if not q_nope.is_cuda:
+        raise RuntimeError(f"{what}: CUDA tensors required (this operator has no CPU path)")
+    index = q_nope.get_device()
+    if not tables_ok(seq_lens, block_table, index):
+        refuse_tables(what, seq_lens, block_table, index)
+    if not caches_ok(ckv_cache, kpe_cache, index):
+        refuse_caches(what, ckv_cache, kpe_cache, index)
+    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_nope.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: q_nope must be [B*n,heads,512] bf16")
+    rows, heads, _ = q_nope.shape
+    if not 1 <= heads <= MAX_HEADS:
+        raise ValueError(f"{what}: 1 to {MAX_HEADS} heads, got {heads}")
+    if q_pe.shape != (rows, heads, KPE) or q_pe.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: q_pe must be [B*n,heads,64] bf16")
+    if output.shape != q_nope.shape or output.dtype != torch.bfloat16 or lse.shape != (rows, heads) \
+            or lse.dtype != torch.float32:
+        raise ValueError(f"{what}: output must be [B*n,heads,512] bf16 and lse [B*n,heads] float32")
+    if not (q_nope.is_contiguous() and q_pe.is_contiguous() and output.is_contiguous() and lse.is_contiguous()):
+        raise ValueError(f"{what}: q_nope, q_pe, output and lse must be contiguous")
+    raise RuntimeError(f"{what}: all tensors must be on cuda:{index}")
 
 
 def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights=None,
@@ -66,39 +103,31 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
     its request; other entries stay as they were."""
-    if not q_nope.is_cuda:
-        raise RuntimeError("paged attention: CUDA tensors required (this operator has no CPU path)")
-    dev = q_nope.device
-    batch, max_pages = check_tables("paged attention", seq_lens, block_table, dev)
-    pages = check_caches("paged attention", ckv_cache, kpe_cache, dev)
-    if q_nope.dim() != 3 or q_nope.shape[2] != CKV or q_nope.dtype != torch.bfloat16:
-        raise ValueError("paged attention: q_nope must be [B*n,heads,512] bf16")
-    rows, heads, _ = q_nope.shape
-    if not 1 <= heads <= MAX_HEADS:
-        raise ValueError(f"paged attention: 1 to {MAX_HEADS} heads, got {heads}")
-    if q_pe.shape != (rows, heads, KPE) or q_pe.dtype != torch.bfloat16:
-        raise ValueError("paged attention: q_pe must be [B*n,heads,64] bf16")
-    if output.shape != q_nope.shape or output.dtype != torch.bfloat16 or lse.shape != (rows, heads) \
-            or lse.dtype != torch.float32:
-        raise ValueError("paged attention: output must be [B*n,heads,512] bf16 and lse [B*n,heads] float32")
-    if not (q_nope.is_contiguous() and q_pe.is_contiguous() and output.is_contiguous() and lse.is_contiguous()):
-        raise ValueError("paged attention: q_nope, q_pe, output and lse must be contiguous")
-    if q_pe.device != dev or output.device != dev or lse.device != dev:
-        raise RuntimeError(f"paged attention: all tensors must be on {dev}")
+    shape, index = q_nope.shape, q_nope.get_device()
+    bf16 = torch.bfloat16
+    if not (index >= 0 and len(shape) == 3 and shape[2] == CKV and 1 <= shape[1] <= MAX_HEADS
+            and q_pe.shape == (shape[0], shape[1], KPE) and output.shape == shape and lse.shape == shape[:2]
+            and q_nope.dtype is bf16 and q_pe.dtype is bf16 and output.dtype is bf16 and lse.dtype is torch.float32
+            and q_nope.is_contiguous() and q_pe.is_contiguous() and output.is_contiguous() and lse.is_contiguous()
+            and q_pe.get_device() == index and output.get_device() == index and lse.get_device() == index
+            and tables_ok(seq_lens, block_table, index) and caches_ok(ckv_cache, kpe_cache, index)):
+        _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, lse)
+    rows, heads, _ = shape
+    batch, max_pages = block_table.shape
     if rows == 0:
         return None
     if batch == 0 or rows % batch:
         raise ValueError(f"paged attention: {rows} query tokens are no multiple of the {batch} requests")
     old = new = old_stride = new_stride = 0
     if new_token_weights is not None:
-        _check_weights("new_token_weights", new_token_weights, batch, max_pages * PAGE, dev)
-        new, new_stride = new_token_weights.data_ptr(), max(new_token_weights.stride(0), new_token_weights.shape[1])
+        new, new_stride = rows_of("paged attention", "new_token_weights", new_token_weights, batch, max_pages * PAGE,
+                                  torch.float32, index)
     if token_weights is not None:
         if new_token_weights is None:
             raise ValueError("paged attention: token_weights without new_token_weights")
-        _check_weights("token_weights", token_weights, batch, max_pages * PAGE, dev)
-        old, old_stride = token_weights.data_ptr(), max(token_weights.stride(0), token_weights.shape[1])
-        if old != new and workspace.overlap(token_weights, new_token_weights) or old == new and old_stride != new_stride:
+        old, old_stride = rows_of("paged attention", "token_weights", token_weights, batch, max_pages * PAGE, torch.float32,
+                                  index)
+        if (old != new or old_stride != new_stride) and workspace.overlap(token_weights, new_token_weights):
             raise ValueError("paged attention: token_weights and new_token_weights overlap without being one tensor")
     if max_pages == 0:
         output.zero_()
@@ -106,16 +135,15 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
         return None
     lib = _lib.load()
     tokens = rows // batch
-    with workspace.device_guard(dev):
-        need = lib.dsa_paged_attn_workspace_bytes(batch, tokens, heads, max_pages, new_token_weights is not None)
-        # a buffer of the call's own: torch's allocator orders it by stream and by graph
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = lib.dsa_paged_attn(
-            q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), kpe_cache.data_ptr(), seq_lens.data_ptr(),
-            block_table.data_ptr(), block_table.stride(0), float(sm_scale), output.data_ptr(), lse.data_ptr(), old,
-            old_stride, new, new_stride, batch, tokens, heads, pages, max_pages, scratch.data_ptr(), need,
-            workspace.status_word(dev).data_ptr(), workspace.stream_handle(dev))
-    _lib.check(rc, "dsa_paged_attn")
+    need = lib.dsa_paged_attn_workspace_bytes(batch, tokens, heads, max_pages, 1 if new else 0)
+    # a buffer of the call's own: torch's allocator orders it by stream and by graph
+    scratch = torch.empty(need, dtype=torch.uint8, device=q_nope.device)
+    rc = workspace.call_on(
+        index, lib.dsa_paged_attn, q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), kpe_cache.data_ptr(),
+        seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), sm_scale, output.data_ptr(), lse.data_ptr(), old,
+        old_stride, new, new_stride, batch, tokens, heads, ckv_cache.shape[0], max_pages, scratch.data_ptr(), need)
+    if rc:
+        _lib.check(rc, "dsa_paged_attn")
     return None
 
 
@@ -123,9 +151,9 @@ def run(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, out
         new_token_weights=None):
     """Value-returning form: allocates the outputs that are not passed; returns (output, lse)."""
     if output is None:
-        output = torch.empty_like(q_nope, memory_format=torch.contiguous_format)
+        output = q_nope.new_empty(tuple(q_nope.shape))
     if lse is None:
-        lse = torch.empty(q_nope.shape[:2], dtype=torch.float32, device=q_nope.device)
+        lse = q_nope.new_empty(tuple(q_nope.shape[:-1]), dtype=torch.float32)
     kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights,
            new_token_weights)
     return output, lse

@@ -6,6 +6,8 @@ CUDA tensors only; enqueued on the current stream.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib, workspace
@@ -21,6 +23,19 @@ def sections(*counts):
     return [axis for axis, n in enumerate(counts) for _ in range(n)]
 
 
+@functools.lru_cache(maxsize=64)
+def _pack(pair_axes, axes):
+    """The axis of every pair in two bits."""
+    if len(pair_axes) != PAIRS:
+        raise ValueError(f"rotary: pair_axes must have {PAIRS} entries")
+    packed = 0
+    for i, axis in enumerate(pair_axes):
+        if not 0 <= axis < axes:
+            raise ValueError(f"rotary: pair {i} asks for axis {axis} of {axes}")
+        packed |= int(axis) << (2 * i)
+    return packed
+
+
 def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe_cache, q_out=None, interleaved=False):
     """Rotate `q_pe` [n,heads,64] (bf16, strided token and head rows allowed, 1 to 128 heads) into `q_out` (contiguous;
     allocated when None; may be q_pe itself where that is contiguous) and return it; rotate `kpe` [n,64] and store it
@@ -32,56 +47,51 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
     else (i, i+32)."""
     if not q_pe.is_cuda:
         raise RuntimeError("rotary: CUDA tensors required (no CPU path)")
-    dev = q_pe.device
-    if q_pe.dim() != 3 or q_pe.shape[2] != 64 or q_pe.dtype != torch.bfloat16 or q_pe.stride(2) != 1:
+    index, bf16, i32 = q_pe.get_device(), torch.bfloat16, torch.int32
+    if q_pe.dim() != 3 or q_pe.shape[2] != 64 or q_pe.dtype is not bf16 or q_pe.stride(2) != 1:
         raise ValueError("rotary: q_pe must be [n,heads,64] bf16 with dense rows")
     n, heads, _ = q_pe.shape
     if not 1 <= heads <= 128:
         raise ValueError(f"rotary: 1 to 128 heads, got {heads}")
-    if ckv.shape != (n, 512) or kpe.shape != (n, 64) or ckv.dtype != torch.bfloat16 or kpe.dtype != torch.bfloat16 \
+    if ckv.shape != (n, 512) or kpe.shape != (n, 64) or ckv.dtype is not bf16 or kpe.dtype is not bf16 \
             or ckv.stride(1) != 1 or kpe.stride(1) != 1:
         raise ValueError("rotary: ckv must be [n,512] and kpe [n,64], bf16 with dense rows")
     if positions.dim() != 2 or not 1 <= positions.shape[0] <= 4 or positions.shape[1] != n \
-            or positions.dtype != torch.int32 or (n > 1 and positions.stride(1) != 1):
+            or positions.dtype is not i32 or (n > 1 and positions.stride(1) != 1):
         raise ValueError("rotary: positions must be [axes,n] int32 with one to four axes and dense rows")
     axes = positions.shape[0]
-    if inv_freq.shape != (PAIRS,) or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+    if inv_freq.dim() != 1 or inv_freq.shape[0] != PAIRS or inv_freq.dtype is not torch.float32 \
+            or not inv_freq.is_contiguous():
         raise ValueError("rotary: inv_freq must be a contiguous [32] float32 tensor")
-    if len(pair_axes) != PAIRS:
-        raise ValueError(f"rotary: pair_axes must have {PAIRS} entries")
-    packed = 0
-    for i, axis in enumerate(pair_axes):
-        if not 0 <= axis < axes:
-            raise ValueError(f"rotary: pair {i} asks for axis {axis} of {axes}")
-        packed |= axis << (2 * i)
-    if slots.shape != (n,) or slots.dtype != torch.int32 or not slots.is_contiguous():
+    packed = _pack(tuple(pair_axes), axes)
+    if slots.dim() != 1 or slots.shape[0] != n or slots.dtype is not i32 or not slots.is_contiguous():
         raise ValueError("rotary: slots must be a contiguous [n] int32 tensor")
     if ckv_cache.shape[-1] != 512 or kpe_cache.shape[-1] != 64 or not ckv_cache.is_contiguous() \
-            or not kpe_cache.is_contiguous() or ckv_cache.dtype != torch.bfloat16 or kpe_cache.dtype != torch.bfloat16:
+            or not kpe_cache.is_contiguous() or ckv_cache.dtype is not bf16 or kpe_cache.dtype is not bf16:
         raise ValueError("rotary: caches must be contiguous bf16 [...,512] / [...,64]")
     num_slots = ckv_cache.numel() // 512
     if kpe_cache.numel() // 64 != num_slots:
         raise ValueError("rotary: ckv_cache and kpe_cache hold different numbers of slots")
     if q_out is None:
-        q_out = torch.empty(n, heads, 64, dtype=torch.bfloat16, device=dev)
-    elif q_out.shape != q_pe.shape or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous():
+        q_out = q_pe.new_empty((n, heads, 64))
+    elif q_out.shape != q_pe.shape or q_out.dtype is not bf16 or not q_out.is_contiguous():
         raise ValueError("rotary: q_out must be a contiguous [n,heads,64] bf16 tensor")
     elif workspace.overlap(q_out, q_pe) and not (q_out.data_ptr() == q_pe.data_ptr() and q_pe.is_contiguous()):
         raise ValueError("rotary: q_out overlaps q_pe without being the same contiguous tensor")
     for t in (ckv, kpe, positions, inv_freq, slots, ckv_cache, kpe_cache, q_out):
-        if t.device != dev:
-            raise RuntimeError(f"rotary: all tensors must be on {dev}")
+        if t.get_device() != index:
+            raise RuntimeError(f"rotary: all tensors must be on cuda:{index}")
     if n == 0:
         return q_out
     # the stride of an axis of one entry says nothing
     one = n == 1
     lib = _lib.load()
-    with workspace.device_guard(dev):
-        rc = lib.dsa_rotary_append(
-            q_pe.data_ptr(), heads * 64 if one else q_pe.stride(0), 64 if heads == 1 else q_pe.stride(1),
-            ckv.data_ptr(), 512 if one else ckv.stride(0), kpe.data_ptr(), 64 if one else kpe.stride(0),
-            positions.data_ptr(), n if axes == 1 else positions.stride(0), axes, inv_freq.data_ptr(), packed,
-            1 if interleaved else 0, slots.data_ptr(), q_out.data_ptr(), ckv_cache.data_ptr(), kpe_cache.data_ptr(), n,
-            heads, num_slots, workspace.status_word(dev).data_ptr(), workspace.stream_handle(dev))
-    _lib.check(rc, "dsa_rotary_append")
+    rc = workspace.call_on(
+        index, lib.dsa_rotary_append, q_pe.data_ptr(), heads * 64 if one else q_pe.stride(0),
+        64 if heads == 1 else q_pe.stride(1), ckv.data_ptr(), 512 if one else ckv.stride(0), kpe.data_ptr(),
+        64 if one else kpe.stride(0), positions.data_ptr(), n if axes == 1 else positions.stride(0), axes,
+        inv_freq.data_ptr(), packed, 1 if interleaved else 0, slots.data_ptr(), q_out.data_ptr(), ckv_cache.data_ptr(),
+        kpe_cache.data_ptr(), n, heads, num_slots)
+    if rc:
+        _lib.check(rc, "dsa_rotary_append")
     return q_out

@@ -46,6 +46,20 @@ def device_guard(device: torch.device):
     return torch.cuda.device(device)
 
 
+def status_address(index: int) -> int:
+    """Device address of `status_word` of the device with this index."""
+    word = _status.get(index)
+    return (word if word is not None else status_word(torch.device("cuda", index))).data_ptr()
+
+
+def call_on(index: int, fn, *args) -> int:
+    """fn(*args, status word, current stream) with the device of this index current."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, status_address(index), _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, status_address(index), _raw_stream(index))
+
+
 def stream_handle(device: torch.device) -> int:
     """cudaStream_t of torch's current stream on `device` (the stream the C ABI enqueues on)."""
     if _raw_stream is not None and device.index is not None:
@@ -55,14 +69,14 @@ def stream_handle(device: torch.device) -> int:
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory spans of two tensors meet (from the first element to the last, gaps included)."""
-    def span(t):
-        if t.numel() == 0:
-            return 0, 0
-        first = t.data_ptr()
-        return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-    a0, a1 = span(a)
-    b0, b1 = span(b)
-    return a0 < b1 and b0 < a1
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa == 0 or pb == 0 or a.numel() == 0 or b.numel() == 0:
+        return False
+    low, first, last = (a, pa, pb) if pa <= pb else (b, pb, pa)
+    span = 1
+    for n, s in zip(low.shape, low.stride()):
+        span += (n - 1) * s
+    return last < first + span * low.element_size()
 
 
 STATUS_BITS = {
