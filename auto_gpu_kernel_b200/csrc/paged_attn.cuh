@@ -9,7 +9,6 @@
 // leaves a partial result.  Lengths live on the device, so every CTA works the split out for itself.
 #pragma once
 
-#include <cstdlib>
 #include "common.cuh"
 
 namespace dsa {
@@ -39,7 +38,7 @@ constexpr int kPagedMaxRanges = 512;
 // Query rows that a CTA takes at once, from the rows of a request: 16 or 32 by warp-level products (one or two row
 // groups per page), 64 by tcgen05.
 inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-inline int paged_switch_cost(int rows) { const char* e = getenv("SWC"); return e ? atoi(e) : (rows <= 32 ? 2 : 4); }
+inline int paged_switch_cost(int rows) { return rows <= 32 ? 3 : 4; }
 
 __host__ __device__ inline int paged_len(int len, int max_pages) {
   const int64_t most = (int64_t)max_pages * kPage;
@@ -50,8 +49,8 @@ __host__ __device__ inline int paged_tiles(int len, int max_pages) {
   return n < 1 ? 1 : n;
 }
 
-// Partial results: per (row block, range, which) a [rows of the block][512] fp32 accumulator ([512][64] for blocks of
-// 64 rows), then its running maxima and sums.  `which` is 1 for the segment a request begins with and 0 for the ones that follow: a range
+// Partial results: per (row block, range, which) a [rows of the block][512] fp32 accumulator ([16][512][4] for blocks of
+// 64 rows: four rows, column, row of the four), then its running maxima and sums.  `which` is 1 for the segment a request begins with and 0 for the ones that follow: a range
 // holds at most one of each.
 __host__ __device__ inline size_t paged_part_floats(int block_rows) { return (size_t)block_rows * (kCkv + 2); }
 __device__ __forceinline__ float* paged_part(const PagedArgs& a, int block_rows, int rb, int range, int which) {
@@ -87,8 +86,12 @@ __device__ __forceinline__ long long paged_scan(const PagedArgs& a, long long* s
 }
 
 // Units of a range, and the unit that request b's tiles begin at when `tiles` tiles lie in front of it.
+// (64-bit divisions are hundreds of instructions, and every thread of a small kernel would make them)
+__device__ __forceinline__ long long paged_div(long long x, long long y) {
+  return x <= 0x7fffffffll && y <= 0x7fffffffll ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
+}
 __device__ __forceinline__ long long paged_units(const PagedArgs& a, long long total) {
-  return (total + (long long)a.batch * a.switch_cost + a.grid_x - 1) / a.grid_x;
+  return paged_div(total + (long long)a.batch * a.switch_cost + a.grid_x - 1, a.grid_x);
 }
 __device__ __forceinline__ long long paged_first_unit(const PagedArgs& a, int b, long long tiles) {
   return tiles + (long long)(b + 1) * a.switch_cost;
@@ -134,16 +137,12 @@ __device__ __forceinline__ void paged_find_segments(const PagedArgs& a, int b, l
   int lo, hi;
   long long before;
   const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
+  if (b < lo || b >= hi) return;
   const long long per = paged_units(a, total);
-  for (int k = lo; k < hi && k <= b; ++k) {
-    const int tiles = paged_tiles(__ldg(a.seq_lens + k), a.max_pages);
-    if (k == b) {
-      const long long first = paged_first_unit(a, b, before);
-      out->first = (int)(first / per);
-      out->count = (int)((first + tiles - 1) / per) - out->first + 1;
-    }
-    before += tiles;
-  }
+  for (int k = lo; k < b; ++k) before += paged_tiles(__ldg(a.seq_lens + k), a.max_pages);
+  const long long first = paged_first_unit(a, b, before);
+  out->first = (int)paged_div(first, per);
+  out->count = (int)paged_div(first + paged_tiles(__ldg(a.seq_lens + b), a.max_pages) - 1, per) - out->first + 1;
 }
 
 }  // namespace dsa

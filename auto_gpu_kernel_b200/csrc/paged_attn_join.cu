@@ -14,32 +14,35 @@ namespace dsa {
 namespace {
 
 // A partial result is an accumulator u, its running maximum and its sum; an empty one has maximum -inf and sum 0, one
-// of NaNs a NaN sum.
-template <int kN>
-__device__ __forceinline__ void join_add(float& m, float& l, float (&v)[kN], float m2, float l2, const float (&u)[kN]) {
+// of NaNs a NaN sum.  What the two accumulators (m, l) and (m2, l2) are multiplied by when they are added:
+__device__ __forceinline__ void join_factors(float& m, float& l, float m2, float l2, float& c, float& f) {
   const float mx = fmaxf(m, m2);
-  const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - mx);
-  const float f = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : exp2f(m2 - mx);
+  c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - mx);
+  f = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : exp2f(m2 - mx);
   m = mx;
   l = l * c + l2 * f;
-#pragma unroll
-  for (int k = 0; k < kN; ++k) v[k] = v[k] * c + u[k] * f;
 }
 
-// Threads share a row's segments out in kSplit groups, each group with a running maximum of its own, and the first
-// adds the groups up through shared memory.  A group's loads do not wait for one another (four segments of them are
-// in flight), so a request with a hundred segments costs a few trips to L2 when enough groups share them.
-//   kColumns false: partial results [row][512]; a CTA has one row and 128 of its columns, a thread four of these
-//   kColumns true:  partial results [512][64] (row blocks of 64); a CTA has 64 rows and eight columns, a thread a row
-template <bool kColumns, int kSplit>
-__global__ void __launch_bounds__(kSplit * (kColumns ? 64 : 32))
+// 32 threads to a group; kSplit groups share the segments out, each with a running maximum of its
+// own, and are then added up, every value by a thread of its own.  A group's loads do not wait for one another (kDepth
+// segments of them are in flight), so a request with a hundred segments costs a few trips to L2 when enough groups
+// share them.
+//   kQuads false: partial results [row][512]; a CTA has one row and 128 of its columns, a thread four of these
+//   kQuads true:  partial results [16][512][4] (row blocks of 64: four rows, column, row of the four); a CTA has four
+//                 rows and 128 columns, a thread four of these, 32 apart
+template <bool kQuads, int kSplit>
+__global__ void __launch_bounds__(kSplit * 32)
 paged_join_kernel(const PagedArgs a) {
-  constexpr int kGroup = kColumns ? 64 : 32, kN = kColumns ? 8 : 4, kThreads = kSplit * kGroup;
-  __shared__ long long sums[kThreads / 32];
+  constexpr int kThreads = kSplit * 32, kDepth = kQuads ? 2 : 5;
+  constexpr int kM = kQuads ? 4 : 1;               // rows of a thread
+  constexpr int kV = 4 * kM;                       // values of a thread: of row k % kM
+  __shared__ long long sums[kSplit];
   __shared__ PagedSegments seg;
-  __shared__ float acc_sh[kSplit > 1 ? kSplit : 1][kN + 2][kGroup];
-  const int tid = threadIdx.x, c = tid % kGroup, grp = tid / kGroup;
-  const int items = kColumns ? (a.rows + 63) / 64 : a.rows;
+  __shared__ float acc_sh[kSplit > 1 ? kSplit : 1][kV][32];      // the groups' values
+  __shared__ float sum_sh[kSplit > 1 ? kSplit : 1][kM];         // their rows' sums and maxima
+  __shared__ float max_sh[kSplit > 1 ? kSplit : 1][kM];
+  const int tid = threadIdx.x, c = tid & 31, grp = tid >> 5;
+  const int items = kQuads ? (a.rows + 3) / 4 : a.rows;
   const int b = (int)(blockIdx.x / items), item = (int)(blockIdx.x % items);
   // lengths are older than the attention kernel, which waits for its own predecessor before it lets this one start
   paged_find_segments<kThreads>(a, b, sums, &seg);
@@ -48,56 +51,109 @@ paged_join_kernel(const PagedArgs a) {
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   if (n_seg == 1) return;               // the attention wrote this request itself
-  const int rb = kColumns ? item : item / a.block_rows, br = kColumns ? c : item - rb * a.block_rows;
-  const int col = blockIdx.y * (kColumns ? 8 : 128) + (kColumns ? 0 : 4 * c);
-  float m = -INFINITY, l = 0.f, v[kN];
+  const int row0 = kQuads ? 4 * item : item, rb = row0 / a.block_rows, br = row0 - rb * a.block_rows;
+  const int col = blockIdx.y * 128 + (kQuads ? c : 4 * c);
+  const size_t place = kQuads ? ((size_t)(br >> 2) * kCkv + col) * 4 : (size_t)br * kCkv + col;
+  float m[kM], l[kM], v[kV];
 #pragma unroll
-  for (int k = 0; k < kN; ++k) v[k] = 0.f;
-#pragma unroll 4
-  for (int s = grp; s < n_seg; s += kSplit) {
-    const float* p = paged_part(a, a.block_rows, rb, x0 + s, s == 0 ? 1 : 0);
-    float u[kN];
-    if (kColumns) {
+  for (int k = 0; k < kV; ++k) v[k] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kN; ++k) u[k] = __ldcg(p + (size_t)(col + k) * 64 + br);
-    } else {
-      const float4 t = __ldcg(reinterpret_cast<const float4*>(p + (size_t)br * kCkv + col));
-      u[0] = t.x;
-      u[1] = t.y;
-      u[2] = t.z;
-      u[3] = t.w;
+  for (int k = 0; k < kM; ++k) {
+    m[k] = -INFINITY;
+    l[k] = 0.f;
+  }
+  for (int s0 = grp; s0 < n_seg; s0 += kSplit * kDepth) {
+    float u[kDepth][kV], m2[kDepth][kM], l2[kDepth][kM];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int s = s0 + d * kSplit;
+#pragma unroll
+      for (int k = 0; k < kV; ++k) u[d][k] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kM; ++k) {
+        m2[d][k] = -INFINITY;
+        l2[d][k] = 0.f;
+      }
+      if (s < n_seg) {
+        const float* p = paged_part(a, a.block_rows, rb, x0 + s, s == 0 ? 1 : 0);
+        const float* stat = p + (size_t)a.block_rows * kCkv + br;
+#pragma unroll
+        for (int q = 0; q < kM; ++q)               // (quads: 32 columns on is 128 floats on)
+          *reinterpret_cast<float4*>(u[d] + 4 * q) = __ldcg(reinterpret_cast<const float4*>(p + place + 128 * q));
+        if constexpr (kQuads) {
+          *reinterpret_cast<float4*>(m2[d]) = __ldcg(reinterpret_cast<const float4*>(stat));
+          *reinterpret_cast<float4*>(l2[d]) = __ldcg(reinterpret_cast<const float4*>(stat + a.block_rows));
+        } else {
+          m2[d][0] = __ldcg(stat);
+          l2[d][0] = __ldcg(stat + a.block_rows);
+        }
+      }
     }
-    const float m2 = __ldcg(p + (size_t)a.block_rows * kCkv + br), l2 = __ldcg(p + (size_t)a.block_rows * (kCkv + 1) + br);
-    join_add(m, l, v, m2, l2, u);
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      float f0[kM], f1[kM];
+#pragma unroll
+      for (int k = 0; k < kM; ++k) join_factors(m[k], l[k], m2[d][k], l2[d][k], f0[k], f1[k]);
+#pragma unroll
+      for (int k = 0; k < kV; ++k) v[k] = v[k] * f0[k % kM] + u[d][k] * f1[k % kM];
+    }
   }
   if (kSplit > 1) {
+    if (c == 0) {
 #pragma unroll
-    for (int k = 0; k < kN; ++k) acc_sh[grp][k][c] = v[k];
-    acc_sh[grp][kN][c] = m;
-    acc_sh[grp][kN + 1][c] = l;
+      for (int k = 0; k < kM; ++k) max_sh[grp][k] = m[k];
+    }
+    __syncthreads();
+    float f[kM];
+#pragma unroll
+    for (int k = 0; k < kM; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int s = 0; s < kSplit; ++s) top = fmaxf(top, max_sh[s][k]);
+      f[k] = m[k] == -INFINITY ? (l[k] == 0.f ? 0.f : 1.f) : exp2f(m[k] - top);
+      m[k] = top;
+      if (c == 0) sum_sh[grp][k] = l[k] * f[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) acc_sh[grp][k][c] = v[k] * f[k % kM];
+    __syncthreads();
+    // in the order of the groups, back into the first group's place
+    for (int i = tid; i < 32 * kV; i += kThreads) {
+      float t = acc_sh[0][i >> 5][i & 31];
+#pragma unroll
+      for (int s = 1; s < kSplit; ++s) t += acc_sh[s][i >> 5][i & 31];
+      acc_sh[0][i >> 5][i & 31] = t;
+    }
     __syncthreads();
     if (grp > 0) return;
-#pragma unroll 4
-    for (int s = 1; s < kSplit; ++s) {
-      float u[kN];
 #pragma unroll
-      for (int k = 0; k < kN; ++k) u[k] = acc_sh[s][k][c];
-      join_add(m, l, v, acc_sh[s][kN][c], acc_sh[s][kN + 1][c], u);
+    for (int k = 0; k < kV; ++k) v[k] = acc_sh[0][k][c];
+#pragma unroll
+    for (int k = 0; k < kM; ++k) {
+      l[k] = sum_sh[0][k];
+#pragma unroll
+      for (int s = 1; s < kSplit; ++s) l[k] += sum_sh[s][k];
     }
   }
-  const int r = kColumns ? rb * 64 + c : item;
-  if (r >= a.rows) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint32_t h[kN / 2];
+  float inv[kM];
 #pragma unroll
-  for (int k = 0; k < kN / 2; ++k) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k] * inv, v[2 * k + 1] * inv);
-    h[k] = *reinterpret_cast<const uint32_t*>(&t);
+  for (int k = 0; k < kM; ++k) inv[k] = l[k] == 0.f ? 0.f : 1.f / l[k];
+  const size_t row = (size_t)b * a.rows + row0;
+  if constexpr (kQuads) {
+#pragma unroll
+    for (int k = 0; k < kV; ++k)
+      if (row0 + k % 4 < a.rows) a.out[(row + k % 4) * kCkv + col + 32 * (k / 4)] = __float2bfloat16_rn(v[k] * inv[k % 4]);
+  } else {
+    const __nv_bfloat162 p0 = __floats2bfloat162_rn(v[0] * inv[0], v[1] * inv[0]);
+    const __nv_bfloat162 p1 = __floats2bfloat162_rn(v[2] * inv[0], v[3] * inv[0]);
+    *reinterpret_cast<uint2*>(a.out + row * kCkv + col) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
   }
-  const size_t row = (size_t)b * a.rows + r;
-  if constexpr (kColumns) *reinterpret_cast<uint4*>(a.out + row * kCkv + col) = make_uint4(h[0], h[1], h[2], h[3]);
-  else *reinterpret_cast<uint2*>(a.out + row * kCkv + col) = make_uint2(h[0], h[1]);
-  if (blockIdx.y == 0 && (kColumns || c == 0)) a.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
+  if (blockIdx.y == 0 && c == 0) {
+#pragma unroll
+    for (int k = 0; k < kM; ++k)
+      if (row0 + k < a.rows) a.lse[row + k] = l[k] == 0.f ? -INFINITY : m[k] + log2f(l[k]);
+  }
 }
 
 // Four cached tokens per thread, 1024 of one request per CTA; a row's 64 logits of a page are one coalesced 256-byte
@@ -162,15 +218,16 @@ cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, cudaS
 }  // namespace
 
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t stream) {
-  // about ranges / requests segments to a request; four loads in flight per group are one trip to L2
+  // about ranges / requests segments to a request; a few loads in flight per group are one trip to L2
   const int seg = a.grid_x / a.batch;
   if (a.block_rows == 64) {
-    const dim3 grid((unsigned)a.batch * (unsigned)((a.rows + 63) / 64), kCkv / 8);
-    if (seg > 16) return launch_after(paged_join_kernel<true, 16>, grid, 16 * 64, stream, a);
-    return launch_after(paged_join_kernel<true, 4>, grid, 4 * 64, stream, a);
+    const dim3 grid((unsigned)a.batch * (unsigned)((a.rows + 3) / 4), kCkv / 128);
+    if (seg > 32) return launch_after(paged_join_kernel<true, 16>, grid, 16 * 32, stream, a);
+    if (seg > 2) return launch_after(paged_join_kernel<true, 2>, grid, 2 * 32, stream, a);
+    return launch_after(paged_join_kernel<true, 1>, grid, 32, stream, a);
   }
   const dim3 grid((unsigned)a.batch * (unsigned)a.rows, kCkv / 128);
-  if (seg > 16) return launch_after(paged_join_kernel<false, 32>, grid, 32 * 32, stream, a);
+  if (seg > 64) return launch_after(paged_join_kernel<false, 16>, grid, 16 * 32, stream, a);
   if (seg > 4) return launch_after(paged_join_kernel<false, 4>, grid, 4 * 32, stream, a);
   return launch_after(paged_join_kernel<false, 1>, grid, 32, stream, a);
 }

@@ -302,7 +302,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
         ptx::named_bar_sync(1, kTcSoftmax);
         ptx::tc_fence_after();
         const int rows_here = min(kTcRows, a.rows - rb * kTcRows);
-        // a lane has an output column, a register a row: partial results stay that way, [column][row]
+        // a lane has an output column, a register a row: partial results are stored four rows at a time, [16][512][4]
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int block = 2 * half + (c >> 1), r0 = 32 * (c & 1);
@@ -321,9 +321,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
             for (int k = 0; k < 32; ++k)
               if (r0 + k < rows_here) dst[(size_t)k * kCkv] = __float2bfloat16_rn(__uint_as_float(o[k]) * sh.inv[r0 + k]);
           } else {
-            uint4* dst = reinterpret_cast<uint4*>(part + (size_t)col * kTcRows + r0);
+            uint4* dst = reinterpret_cast<uint4*>(part) + (size_t)(r0 >> 2) * kCkv + col;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 8; ++k)
+              dst[(size_t)k * kCkv] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
         ptx::tc_fence_before();

@@ -9,6 +9,8 @@ up how much attention every cached token received, which `cache_evict` chooses b
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib, workspace
@@ -91,6 +93,12 @@ def _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, l
     raise RuntimeError(f"{what}: all tensors must be on cuda:{index}")
 
 
+@functools.lru_cache(maxsize=512)
+def _workspace_bytes(index, batch, tokens, heads, max_pages, with_weights):
+    with torch.cuda.device(index):
+        return _lib.load().dsa_paged_attn_workspace_bytes(batch, tokens, heads, max_pages, with_weights)
+
+
 def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights=None,
            new_token_weights=None):
     """Write the attention output and the base-2 LSE in place; enqueued on the current stream, returns None.
@@ -135,7 +143,7 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
         return None
     lib = _lib.load()
     tokens = rows // batch
-    need = lib.dsa_paged_attn_workspace_bytes(batch, tokens, heads, max_pages, 1 if new else 0)
+    need = _workspace_bytes(index, batch, tokens, heads, max_pages, 1 if new else 0)
     # a buffer of the call's own: torch's allocator orders it by stream and by graph
     scratch = torch.empty(need, dtype=torch.uint8, device=q_nope.device)
     rc = workspace.call_on(
