@@ -35,10 +35,12 @@ struct PagedArgs {
 
 constexpr int kPagedMaxRanges = 512;
 
-// Query rows that a CTA takes at once, from the rows of a request: 16 or 32 by warp-level products (one or two row
-// groups per page), 64 by tcgen05.
-inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-inline int paged_switch_cost(int rows) { return rows <= 32 ? 3 : 4; }
+// Query rows that a CTA takes at once, from the rows of a request: 16 by warp-level products, 64 by tcgen05.  At 16 rows the
+// two are equally fast on long caches and the first starts sooner (TODO); from 17 on the second reads the cache once
+// where the first would read it twice.
+inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : 64; }
+// What taking up a request costs, in tiles.
+inline int paged_switch_cost(int rows) { return rows <= 16 ? 3 : 2; }
 
 __host__ __device__ inline int paged_len(int len, int max_pages) {
   const int64_t most = (int64_t)max_pages * kPage;

@@ -1,4 +1,5 @@
-// Dense attention of every request's newest tokens over its whole paged ckv / kpe cache.
+// Dense attention of every request's newest tokens over its whole paged ckv / kpe cache, for requests of at most 16 query
+// rows (one new token of 16 heads); paged_attn_tc.cu has the others.
 //
 //   x[r,k]  = (q_nope[r].ckv[k] + q_pe[r].kpe[k]) * sm_scale * log2 e        k < the positions row r sees
 //   lse[r]  = log2 sum_k 2^x[r,k]        out[r] = sum_k 2^(x[r,k] - lse[r]) ckv[k]
@@ -12,13 +13,12 @@
 // ckv column blocks and kpe) with the 128-byte swizzle, which keeps both ldmatrix patterns free of bank conflicts;
 // nine lanes of warp 0 issue a page's boxes two pages ahead, into the stage that the page before the current one has
 // just left, and look the page ids up 32 at a time, one batch ahead.
-//   S = Q.K^T   warp w has the 16-row group w % MT of the block and 8 MT of the page's tokens; q_nope stays in
-//               registers as 32 A fragments, q_pe in shared memory (all 36 left the loop no registers to schedule in);
+//   S = Q.K^T   warp w has tokens 8w .. 8w+7 of the page; q_nope stays in registers as 32 A fragments, q_pe in shared
+//               memory (all 36 in registers left the loop none to schedule in);
 //   softmax     base 2, the running maximum refreshed (and O rescaled) only when a logit exceeds it by more than 2^8;
 //               P is rounded to bf16 for the second product, as the cache that it multiplies is bf16; sums are taken
 //               of the fp32 values;
-//   O += P.V    warp w has the output columns 64w .. 64w+63 = column block w of the same stage (ldmatrix.trans), for
-//               all MT row groups.
+//   O += P.V    warp w has the output columns 64w .. 64w+63 = column block w of the same stage (ldmatrix.trans).
 // Rows behind a request's length are put to zero in the stage before the second product: the cache may hold anything
 // there, and 0 x NaN would get into the sum.
 #include "mma.cuh"
@@ -34,6 +34,7 @@ constexpr int kPaStages = 3;
 constexpr int kPaBlockBytes = kPage * 128;           // 8192
 constexpr int kPaStageBytes = 9 * kPaBlockBytes;     // 73728
 constexpr int kPaThreads = 256;
+constexpr int kPaRows = 16;                          // query rows of a block
 constexpr int kPaQPitch = 1040;                      // 1024-byte q_nope rows, padded against bank conflicts
 constexpr float kPaRescaleGap = 8.f;
 
@@ -43,22 +44,18 @@ struct PaTile {
 struct PaShared {
   uint64_t full[kPaStages];
   PaTile tile[kPaStages];
-  float red[8 * kHeads];        // [token group][block row]
+  float red[8][kPaRows];
   long long sums[kPaThreads / 32];
   PagedRange range;
 };
 
-template <int MT>
-constexpr size_t pa_dyn_bytes() {
-  return 1024 + kPaStages * kPaStageBytes + 2 * 16 * MT * 128 + sizeof(PaShared);
-}
+constexpr size_t kPaDynBytes = 1024 + kPaStages * kPaStageBytes + 2 * kPaRows * 128 + sizeof(PaShared);
+static_assert(kPaDynBytes <= 232448, "shared memory of one CTA");
 
-template <int MT, bool kLogits>
+template <bool kLogits>
 __global__ void __launch_bounds__(kPaThreads, 1)
 paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_constant__ CUtensorMap map_kpe,
                       const PagedArgs a) {
-  constexpr int kRows = 16 * MT;            // rows of a block
-  constexpr int kGroups = 8 / MT;           // token groups
   extern __shared__ unsigned char dyn_raw[];
   const uint32_t raw_addr = smem_u32(dyn_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -66,12 +63,11 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
   unsigned char* kv_ptr = dyn_raw + pad;
   const uint32_t p_addr = kv_addr + kPaStages * kPaStageBytes;
   unsigned char* p_ptr = kv_ptr + kPaStages * kPaStageBytes;
-  const uint32_t qpe_addr = p_addr + kRows * 128;
-  PaShared& sh = *reinterpret_cast<PaShared*>(p_ptr + 2 * kRows * 128);
+  const uint32_t qpe_addr = p_addr + kPaRows * 128;
+  PaShared& sh = *reinterpret_cast<PaShared*>(p_ptr + 2 * kPaRows * 128);
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  const int mt = w % MT, tg = w / MT;
   const int rb = blockIdx.y, range = blockIdx.x;
 
   if (tid == 0) {
@@ -144,9 +140,9 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
 
   // q rows of a request's block, padded rows as zeros
   auto stage_q = [&](int b, uint32_t qs) {
-    for (int c = tid; c < kRows * 72; c += kPaThreads) {
+    for (int c = tid; c < kPaRows * 72; c += kPaThreads) {
       const int h = c / 72, jj = c - h * 72;
-      const int r = rb * kRows + h;
+      const int r = rb * kPaRows + h;
       const size_t row = (size_t)b * a.rows + (r < a.rows ? r : 0);
       const __nv_bfloat16* src = jj < 64 ? a.q_nope + row * kCkv + jj * 8 : a.q_pe + row * kKpe + (jj - 64) * 8;
       const uint32_t dst = jj < 64 ? qs + h * kPaQPitch + jj * 16 : qpe_addr + h * 128 + (((jj - 64) ^ (h & 7)) << 4);
@@ -162,23 +158,20 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
 
   // where the logits of a tile go (only where they are wanted)
   auto tile_logits = [&](const PaTile& t) {
-    return a.logits + (((size_t)t.b * a.max_pages + t.j) * gridDim.y + rb) * (size_t)(kRows * kPage);
+    return a.logits + (((size_t)t.b * a.max_pages + t.j) * gridDim.y + rb) * (size_t)(kPaRows * kPage);
   };
   // token (of the request's new ones) of each row of this thread; rows behind the last see nothing
-  int row_tok[MT][2];
+  int row_tok[2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = rb * kRows + 16 * m + g + 8 * e;
-      row_tok[m][e] = r < a.rows ? r / a.heads : -1;
-    }
+  for (int e = 0; e < 2; ++e) {
+    const int r = rb * kPaRows + g + 8 * e;
+    row_tok[e] = r < a.rows ? r / a.heads : -1;
   }
 
   uint32_t qa[32][4];           // A fragments of q_nope: k-step ks covers columns 16 ks .. 16 ks + 15
-  float o[MT][8][4];            // O[rows 16m+g / +8][columns 64 w + 8 n + 2 t4, +1]
-  float m_run[MT][2];           // running maxima of all rows of the block that this thread accumulates
-  float l0 = 0.f, l1 = 0.f;     // row sums over this thread's tokens, rows of group mt
+  float o[8][4];                // O[rows g / g+8][columns 64 w + 8 n + 2 t4, +1]
+  float m0 = -INFINITY, m1 = -INFINITY;
+  float l0 = 0.f, l1 = 0.f;     // row sums over this thread's tokens
   int cur_b = -1, first_j = 0, lim0 = 0, lim1 = 0;
   bool lost = false;
 
@@ -197,23 +190,18 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       if (i > 0) stage_q(tile.b, qs);
       cp_async_wait_group<0>();
       __syncthreads();
-      const uint32_t qrow = qs + (16 * mt + (lane & 7) + ((lane >> 3) & 1) * 8) * kPaQPitch + (lane >> 4) * 16;
+      const uint32_t qrow = qs + ((lane & 7) + ((lane >> 3) & 1) * 8) * kPaQPitch + (lane >> 4) * 16;
 #pragma unroll
       for (int ks = 0; ks < 32; ++ks) ldsm_x4(qrow + ks * 32, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        m_run[m][0] = m_run[m][1] = -INFINITY;
-#pragma unroll
-        for (int nn = 0; nn < 8; ++nn) o[m][nn][0] = o[m][nn][1] = o[m][nn][2] = o[m][nn][3] = 0.f;
-      }
+      for (int nn = 0; nn < 8; ++nn) o[nn][0] = o[nn][1] = o[nn][2] = o[nn][3] = 0.f;
+      m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
       cur_b = tile.b;
       first_j = tile.j;
       const int base = tile.len - a.tokens + 1;
-      int k0 = row_tok[0][0], k1 = row_tok[0][1];
-      if (MT > 1 && mt) { k0 = row_tok[MT - 1][0]; k1 = row_tok[MT - 1][1]; }
-      lim0 = k0 < 0 ? 0 : base + k0;
-      lim1 = k1 < 0 ? 0 : base + k1;
+      lim0 = row_tok[0] < 0 ? 0 : base + row_tok[0];
+      lim1 = row_tok[1] < 0 ? 0 : base + row_tok[1];
       ptx::fence_proxy_async_smem();   // the stage now goes back from plain stores and reads to TMA
       __syncthreads();
     }
@@ -222,7 +210,7 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
     if (!tile.live) {
       if (kLogits && tile.len > 0) {
         float* lg = tile_logits(tile);
-        for (int c = tid; c < kRows * kPage; c += kPaThreads) lg[c] = -INFINITY;
+        for (int c = tid; c < kPaRows * kPage; c += kPaThreads) lg[c] = -INFINITY;
       }
     } else {
       const uint32_t sa = kv_addr + s * kPaStageBytes;
@@ -235,73 +223,56 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
         }
         ptx::fence_proxy_async_smem();   // TMA writes the stage next
       }
-      // ---- S = Q . K^T for tokens 8 MT tg .. + 8 MT - 1; four accumulator chains ----------------
+      // ---- S = Q . K^T for tokens 8w .. 8w+7; four accumulator chains --------------------------
       float acc[4][4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int tok = 8 * (MT * tg + t) + (lane & 7);
+      {
+        const int tok = 8 * w + (lane & 7), rx = tok & 7, quad = lane >> 3;
         const uint32_t brow = sa + tok * 128;
-        const int rx = tok & 7, quad = lane >> 3;
 #pragma unroll
         for (int kb = 0; kb < 9; ++kb) {
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             uint32_t r0, r1, r2, r3;
             ldsm_x4(brow + kb * kPaBlockBytes + (((kk * 4 + quad) ^ rx) << 4), r0, r1, r2, r3);
-            const int c = MT == 1 ? 2 * kk : 2 * t;
             if (kb < 8) {
-              hmma_16816(acc[c], qa[kb * 4 + 2 * kk], r0, r1);
-              hmma_16816(acc[c + 1], qa[kb * 4 + 2 * kk + 1], r2, r3);
+              hmma_16816(acc[2 * kk], qa[kb * 4 + 2 * kk], r0, r1);
+              hmma_16816(acc[2 * kk + 1], qa[kb * 4 + 2 * kk + 1], r2, r3);
             } else {                     // q_pe
-              const int qr = 16 * mt + (lane & 7) + ((lane >> 3) & 1) * 8;
+              const int qr = (lane & 7) + ((lane >> 3) & 1) * 8;
               uint32_t qp[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 ldsm_x4(qpe_addr + qr * 128 + (((4 * kk + 2 * h + (lane >> 4)) ^ (qr & 7)) << 4), qp[h][0], qp[h][1], qp[h][2],
                         qp[h][3]);
-              hmma_16816(acc[c], qp[0], r0, r1);
-              hmma_16816(acc[c + 1], qp[1], r2, r3);
+              hmma_16816(acc[2 * kk], qp[0], r0, r1);
+              hmma_16816(acc[2 * kk + 1], qp[1], r2, r3);
             }
           }
         }
       }
-      float x[MT][4];
-      uint32_t* pw[MT][2];              // where this thread's P goes: [row][token], 16-byte chunks swizzled by the row
+      float x[4];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int chunk = MT * tg + t, pa = pos0 + 8 * chunk + 2 * t4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = MT == 1 ? (acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e]) : acc[2 * t][e] + acc[2 * t + 1][e];
-          const bool seen = pa + (e & 1) < (e < 2 ? lim0 : lim1);
-          x[t][e] = seen ? v * a.scale_log2 : -INFINITY;
-        }
-        const int r0 = 16 * mt + g;
-        pw[t][0] = reinterpret_cast<uint32_t*>(p_ptr + r0 * 128 + ((chunk ^ (g & 7)) << 4) + t4 * 4);
-        pw[t][1] = reinterpret_cast<uint32_t*>(p_ptr + (r0 + 8) * 128 + ((chunk ^ (g & 7)) << 4) + t4 * 4);
+      for (int e = 0; e < 4; ++e) {
+        const bool seen = pos0 + 8 * w + 2 * t4 + (e & 1) < (e < 2 ? lim0 : lim1);
+        const float v = (acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e]);
+        x[e] = seen ? v * a.scale_log2 : -INFINITY;
       }
-      float v0 = fmaxf(x[0][0], x[0][1]), v1 = fmaxf(x[0][2], x[0][3]);
-#pragma unroll
-      for (int t = 1; t < MT; ++t) {
-        v0 = fmaxf(v0, fmaxf(x[t][0], x[t][1]));
-        v1 = fmaxf(v1, fmaxf(x[t][2], x[t][3]));
-      }
-      float mm0 = MT > 1 && mt ? m_run[MT - 1][0] : m_run[0][0], mm1 = MT > 1 && mt ? m_run[MT - 1][1] : m_run[0][1];
-      const bool need = v0 > mm0 + kPaRescaleGap || v1 > mm1 + kPaRescaleGap;
-      float p[MT][4];
+      // where this thread's P goes: [row][token], 16-byte chunks swizzled by the row
+      uint32_t* pw0 = reinterpret_cast<uint32_t*>(p_ptr + g * 128 + ((w ^ (g & 7)) << 4) + t4 * 4);
+      uint32_t* pw1 = reinterpret_cast<uint32_t*>(p_ptr + (g + 8) * 128 + ((w ^ (g & 7)) << 4) + t4 * 4);
+      float v0 = fmaxf(x[0], x[1]), v1 = fmaxf(x[2], x[3]);
+      const bool need = v0 > m0 + kPaRescaleGap || v1 > m1 + kPaRescaleGap;
+      float p[4];
       auto publish = [&]() {
-        const float u0 = mm0 == -INFINITY ? 0.f : mm0, u1 = mm1 == -INFINITY ? 0.f : mm1;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          p[t][0] = exp2f(x[t][0] - u0);
-          p[t][1] = exp2f(x[t][1] - u0);
-          p[t][2] = exp2f(x[t][2] - u1);
-          p[t][3] = exp2f(x[t][3] - u1);
-          *pw[t][0] = pack_bf162(p[t][0], p[t][1]);
-          *pw[t][1] = pack_bf162(p[t][2], p[t][3]);
-        }
+        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+        p[0] = exp2f(x[0] - u0);
+        p[1] = exp2f(x[1] - u0);
+        p[2] = exp2f(x[2] - u1);
+        p[3] = exp2f(x[3] - u1);
+        *pw0 = pack_bf162(p[0], p[1]);
+        *pw1 = pack_bf162(p[2], p[3]);
       };
       // P with the running maxima as they are; the barrier that makes it visible tells whether a logit exceeded
       // its maximum by more than 2^8 (rare)
@@ -312,50 +283,37 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
         v1 = fmaxf(v1, __shfl_xor_sync(0xffffffffu, v1, 1));
         v1 = fmaxf(v1, __shfl_xor_sync(0xffffffffu, v1, 2));
         if (t4 == 0) {
-          sh.red[tg * kRows + 16 * mt + g] = v0;
-          sh.red[tg * kRows + 16 * mt + g + 8] = v1;
+          sh.red[w][g] = v0;
+          sh.red[w][g + 8] = v1;
         }
         __syncthreads();
+        float n0 = m0, n1 = m1;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          float c[2];
+        for (int k = 0; k < 8; ++k) {
+          n0 = fmaxf(n0, sh.red[k][g]);
+          n1 = fmaxf(n1, sh.red[k][g + 8]);
+        }
+        const float c0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), c1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= c0;
+        l1 *= c1;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = m_run[m][e];
-#pragma unroll
-            for (int k = 0; k < kGroups; ++k) mx = fmaxf(mx, sh.red[k * kRows + 16 * m + g + 8 * e]);
-            c[e] = mx == -INFINITY ? 1.f : exp2f(m_run[m][e] - mx);
-            m_run[m][e] = mx;
-          }
-#pragma unroll
-          for (int nn = 0; nn < 8; ++nn) {
-            o[m][nn][0] *= c[0];
-            o[m][nn][1] *= c[0];
-            o[m][nn][2] *= c[1];
-            o[m][nn][3] *= c[1];
-          }
-          if (m == mt) {
-            l0 *= c[0];
-            l1 *= c[1];
-            mm0 = m_run[m][0];
-            mm1 = m_run[m][1];
-          }
+        for (int nn = 0; nn < 8; ++nn) {
+          o[nn][0] *= c0;
+          o[nn][1] *= c0;
+          o[nn][2] *= c1;
+          o[nn][3] *= c1;
         }
         publish();
         __syncthreads();
       }
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        l0 += p[t][0] + p[t][1];
-        l1 += p[t][2] + p[t][3];
-      }
+      l0 += p[0] + p[1];
+      l1 += p[2] + p[3];
       if (kLogits) {                    // behind the barrier that the other warps wait at
-        float* lg = tile_logits(tile) + (16 * mt + g) * kPage + 8 * MT * tg + 2 * t4;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          *reinterpret_cast<float2*>(lg + 8 * t) = make_float2(x[t][0], x[t][1]);
-          *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * t) = make_float2(x[t][2], x[t][3]);
-        }
+        float* lg = tile_logits(tile) + g * kPage + 8 * w + 2 * t4;
+        *reinterpret_cast<float2*>(lg) = make_float2(x[0], x[1]);
+        *reinterpret_cast<float2*>(lg + 8 * kPage) = make_float2(x[2], x[3]);
       }
       // ---- O += P . V for columns 64w .. 64w+63 (column block w of the tile) ---------------------
       {
@@ -363,22 +321,16 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
         const uint32_t vbase = sa + w * kPaBlockBytes;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          uint32_t pf[MT][4];
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            ldsm_x4(p_addr + (16 * m + hrow) * 128 + (((ks * 2 + half) ^ (hrow & 7)) << 4), pf[m][0], pf[m][1], pf[m][2],
-                    pf[m][3]);
+          uint32_t pf[4];
+          ldsm_x4(p_addr + hrow * 128 + (((ks * 2 + half) ^ (hrow & 7)) << 4), pf[0], pf[1], pf[2], pf[3]);
           const int vrow = ks * 16 + hrow;
           const uint32_t va = vbase + vrow * 128;
 #pragma unroll
           for (int np = 0; np < 4; ++np) {
             uint32_t r0, r1, r2, r3;
             ldsm_x4_trans(va + (((np * 2 + half) ^ (vrow & 7)) << 4), r0, r1, r2, r3);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              hmma_16816(o[m][2 * np], pf[m], r0, r1);
-              hmma_16816(o[m][2 * np + 1], pf[m], r2, r3);
-            }
+            hmma_16816(o[2 * np], pf, r0, r1);
+            hmma_16816(o[2 * np + 1], pf, r2, r3);
           }
         }
       }
@@ -393,40 +345,37 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       s1 += __shfl_xor_sync(0xffffffffu, s1, 2);
       __syncthreads();                 // sh.red may still be read by a slow warp of a refresh above
       if (t4 == 0) {
-        sh.red[tg * kRows + 16 * mt + g] = s0;
-        sh.red[tg * kRows + 16 * mt + g + 8] = s1;
+        sh.red[w][g] = s0;
+        sh.red[w][g + 8] = s1;
       }
       __syncthreads();
       const bool whole = ends && first_j == 0;
-      float* part = whole ? nullptr : paged_part(a, kRows, rb, range, first_j == 0 ? 1 : 0);
+      float* part = whole ? nullptr : paged_part(a, kPaRows, rb, range, first_j == 0 ? 1 : 0);
       const int col = 64 * w + 2 * t4;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
+      for (int e = 0; e < 2; ++e) {
+        const int br = g + 8 * e, r = rb * kPaRows + br;
+        const float m = e ? m1 : m0;
+        float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int br = 16 * m + g + 8 * e, r = rb * kRows + br;
-          float sum = 0.f;
+        for (int k = 0; k < 8; ++k) sum += sh.red[k][br];
+        if (r >= a.rows) continue;
+        if (whole) {
+          // a row that sees nothing has output 0 and lse -inf; a NaN sum stays NaN
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          __nv_bfloat16* dst = a.out + ((size_t)tile.b * a.rows + r) * kCkv + col;
 #pragma unroll
-          for (int k = 0; k < kGroups; ++k) sum += sh.red[k * kRows + br];
-          if (r >= a.rows) continue;
-          if (whole) {
-            // a row that sees nothing has output 0 and lse -inf; a NaN sum stays NaN
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            __nv_bfloat16* dst = a.out + ((size_t)tile.b * a.rows + r) * kCkv + col;
+          for (int nn = 0; nn < 8; ++nn)
+            *reinterpret_cast<uint32_t*>(dst + 8 * nn) = pack_bf162(o[nn][2 * e] * inv, o[nn][2 * e + 1] * inv);
+          if (w == 0 && t4 == 0) a.lse[(size_t)tile.b * a.rows + r] = sum == 0.f ? -INFINITY : m + log2f(sum);
+        } else {
+          float* dst = part + (size_t)br * kCkv + col;
 #pragma unroll
-            for (int nn = 0; nn < 8; ++nn)
-              *reinterpret_cast<uint32_t*>(dst + 8 * nn) = pack_bf162(o[m][nn][2 * e] * inv, o[m][nn][2 * e + 1] * inv);
-            if (w == 0 && t4 == 0)
-              a.lse[(size_t)tile.b * a.rows + r] = sum == 0.f ? -INFINITY : m_run[m][e] + log2f(sum);
-          } else {
-            float* dst = part + (size_t)br * kCkv + col;
-#pragma unroll
-            for (int nn = 0; nn < 8; ++nn)
-              *reinterpret_cast<float2*>(dst + 8 * nn) = make_float2(o[m][nn][2 * e], o[m][nn][2 * e + 1]);
-            if (w == 0 && t4 == 0) {
-              part[(size_t)kRows * kCkv + br] = sum == 0.f ? -INFINITY : m_run[m][e];
-              part[(size_t)kRows * (kCkv + 1) + br] = sum;
-            }
+          for (int nn = 0; nn < 8; ++nn)
+            *reinterpret_cast<float2*>(dst + 8 * nn) = make_float2(o[nn][2 * e], o[nn][2 * e + 1]);
+          if (w == 0 && t4 == 0) {
+            part[(size_t)kPaRows * kCkv + br] = sum == 0.f ? -INFINITY : m;
+            part[(size_t)kPaRows * (kCkv + 1) + br] = sum;
           }
         }
       }
@@ -441,23 +390,23 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
 
 }  // namespace
 
-template <int MT, bool kLogits>
-static cudaError_t launch_one(const PagedArgs& a, const CUtensorMap& mc, const CUtensorMap& mk, int blocks, cudaStream_t stream) {
+template <bool kLogits>
+static cudaError_t launch_mma(const PagedArgs& a, const CUtensorMap& mc, const CUtensorMap& mk, cudaStream_t stream) {
   static std::atomic<uint64_t> opted{0};
   const cudaError_t e =
-      opt_in_dynamic_smem(reinterpret_cast<const void*>(paged_attn_mma_kernel<MT, kLogits>), pa_dyn_bytes<MT>(), opted);
+      opt_in_dynamic_smem(reinterpret_cast<const void*>(paged_attn_mma_kernel<kLogits>), kPaDynBytes, opted);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.grid_x, (unsigned)blocks);
+  cfg.gridDim = dim3((unsigned)a.grid_x, (unsigned)((a.rows + kPaRows - 1) / kPaRows));
   cfg.blockDim = dim3(kPaThreads);
-  cfg.dynamicSmemBytes = pa_dyn_bytes<MT>();
+  cfg.dynamicSmemBytes = kPaDynBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attn_mma_kernel<MT, kLogits>, mc, mk, a);
+  return cudaLaunchKernelEx(&cfg, paged_attn_mma_kernel<kLogits>, mc, mk, a);
 }
 
 cudaError_t launch_paged_attn_mma(const PagedArgs& a, const void* ckv, const void* kpe, cudaStream_t stream) {
@@ -466,10 +415,7 @@ cudaError_t launch_paged_attn_mma(const PagedArgs& a, const void* ckv, const voi
   if (!make_tmap_2d_sw128(&mc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ckv, kCkv, slots, 64, kPage) ||
       !make_tmap_2d_sw128(&mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kpe, kKpe, slots, 64, kPage))
     return cudaErrorInvalidValue;
-  const int blocks = (a.rows + a.block_rows - 1) / a.block_rows;
-  if (a.block_rows == 16)
-    return a.logits ? launch_one<1, true>(a, mc, mk, blocks, stream) : launch_one<1, false>(a, mc, mk, blocks, stream);
-  return a.logits ? launch_one<2, true>(a, mc, mk, blocks, stream) : launch_one<2, false>(a, mc, mk, blocks, stream);
+  return a.logits ? launch_mma<true>(a, mc, mk, stream) : launch_mma<false>(a, mc, mk, stream);
 }
 
 }  // namespace dsa

@@ -15,7 +15,8 @@
 // their own -- the first product follows the groups as they land, the second hands each back as it is done --
 // and the producer asks L2 for the pages that have no place yet.
 //
-// Roles (320 threads): warps 0-7 softmax and epilogue, warp 8 issues the products, warp 9 the TMA loads.  Every wait is
+// Roles (352 threads): warps 0-7 softmax and epilogue, warp 8 issues the first products and warp 9 the second ones (a
+// second product is not to wait behind a first one whose page is still landing), warp 10 the TMA loads.  Every wait is
 // bounded; a wait that runs out is told at the softmax warps' next barrier, so that all of them leave together, and
 // to the other roles by a flag.
 #include "paged_attn.cuh"
@@ -30,7 +31,7 @@ constexpr int kTcRows = 64;
 constexpr int kTcBlock = kPage * 128;            // one [64 x 128 B] block
 constexpr int kTcPage = 9 * kTcBlock;            // 73728
 constexpr int kTcSoftmax = 256;                 // threads of the softmax warps
-constexpr int kTcThreads = kTcSoftmax + 64;
+constexpr int kTcThreads = kTcSoftmax + 96;
 constexpr int kTcGroups = 4;                     // column groups of a page: ckv blocks 2c, 2c+1; the last also kpe
 constexpr int kTcAhead = 2;                      // pages that L2 is asked for beyond the one being loaded
 constexpr int kTcCols = 512;
@@ -44,7 +45,7 @@ struct TcTile {
   short live, last;     // has a page; is the request's last tile
 };
 struct TcShared {
-  uint64_t full[2][kTcGroups], empty[2][kTcGroups], q_full, q_empty, s_full[2], s_empty[2], p_full, p_empty;
+  uint64_t full[2][kTcGroups], empty[2][kTcGroups], q_full, q_empty, s_full[2], s_empty[2], p_full, p_empty, told;
   TcTile tile[2];
   float corr[kTcRows], inv[kTcRows];   // of each row: what O^T is multiplied by in a refresh, and at the end
   float half[2][kTcRows];              // maxima, at the end sums, over the token halves
@@ -88,6 +89,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
       ptx::mbar_init(smem_u32(&sh.q_empty), 1);
       ptx::mbar_init(smem_u32(&sh.p_full), 8);
       ptx::mbar_init(smem_u32(&sh.p_empty), 1);
+      ptx::mbar_init(smem_u32(&sh.told), 8);
       sh.abort_flag = 0;
       ptx::fence_barrier_init();
     }
@@ -123,11 +125,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
     auto wait = [&](uint64_t& bar, uint32_t parity) {
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(smem_u32(&bar), parity) ? 1 : 0)) lost = 2;
     };
-    auto tell = [&](int which, int flags) {
-      if (lane == 0) sh.word[which][warp] = flags | lost;
-      ptx::named_bar_sync(1, kTcSoftmax);
+    auto words = [&](int which) {
       const int4 u = *reinterpret_cast<const int4*>(&sh.word[which][0]), v = *reinterpret_cast<const int4*>(&sh.word[which][4]);
       return (u.x | u.y | u.z | u.w) | (v.x | v.y | v.z | v.w);
+    };
+    auto tell = [&](int which) {
+      if (lane == 0) sh.word[which][warp] = lost;
+      ptx::named_bar_sync(1, kTcSoftmax);
+      return words(which);
     };
     for (int i = 0; i < n; ++i) {
       const int s = i & 1, phase = (i >> 1) & 1;
@@ -172,8 +177,36 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
         ptx::mbar_arrive(smem_u32(&sh.s_empty[s]));
         ptx::mbar_arrive(smem_u32(&sh.empty[s][0]));
       }
+      // whether a logit exceeds its row's maximum by more than 2^8 is told while the weights are being computed with the
+      // maxima as they are; it is rare
       const bool need = __any_sync(0xffffffffu, v0 > m0 + kTcGap || v1 > m1 + kTcGap);
-      const int told = tell(i & 1, need ? 1 : 0);
+      if (lane == 0) {
+        sh.word[i & 1][warp] = (need ? 1 : 0) | lost;
+        ptx::mbar_arrive(smem_u32(&sh.told));
+      }
+      uint32_t pk[8];
+      float s0, s1;
+      auto weigh = [&]() {
+        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+        s0 = s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p0 = ptx::exp2_ftz(x[4 * k] - u0), p1 = ptx::exp2_ftz(x[4 * k + 1] - u0);
+          const float p2 = ptx::exp2_ftz(x[4 * k + 2] - u1), p3 = ptx::exp2_ftz(x[4 * k + 3] - u1);
+          s0 += p0 + p1;
+          s1 += p2 + p3;
+          const __nv_bfloat162 ha = __floats2bfloat162_rn(p0, p1), hb = __floats2bfloat162_rn(p2, p3);
+          pk[2 * k] = *reinterpret_cast<const uint32_t*>(&ha);
+          pk[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+        }
+      };
+      if (live) weigh();
+      // (every warp arrives within its own waits' limits, far below this one)
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(smem_u32(&sh.told), i & 1, 4000000000ull) ? 1 : 0)) {
+        lost = 2;
+        break;
+      }
+      const int told = words(i & 1);
       if (told & 2) break;
       if (!live) {
         if (kLogits && tile.len > 0) {
@@ -211,7 +244,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
           }
           // the product of the tile before is complete once its P has been handed back
           if (seg_live > 0) wait(sh.p_empty, (pl - 1) & 1);
-          if (tell(2, 0) & 2) break;
+          if (tell(2) & 2) break;
           const float n0 = fmaxf(m0, fmaxf(sh.half[0][row0], sh.half[1][row0]));
           const float n1 = fmaxf(m1, fmaxf(sh.half[0][row0 + 8], sh.half[1][row0 + 8]));
           const float c0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), c1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
@@ -239,19 +272,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
           }
+          weigh();
         }
-        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
-        uint32_t pk[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float p0 = ptx::exp2_ftz(x[4 * k] - u0), p1 = ptx::exp2_ftz(x[4 * k + 1] - u0);
-          const float p2 = ptx::exp2_ftz(x[4 * k + 2] - u1), p3 = ptx::exp2_ftz(x[4 * k + 3] - u1);
-          l0 += p0 + p1;
-          l1 += p2 + p3;
-          const __nv_bfloat162 ha = __floats2bfloat162_rn(p0, p1), hb = __floats2bfloat162_rn(p2, p3);
-          pk[2 * k] = *reinterpret_cast<const uint32_t*>(&ha);
-          pk[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hb);
-        }
+        l0 += s0;
+        l1 += s1;
         // the one P buffer is free once the product of the last tile has read it
         if (pl > 0) wait(sh.p_empty, (pl - 1) & 1);
         unsigned char* pr = p_ptr + row0 * 128 + 4 * t4;
@@ -283,7 +307,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
           sh.half[half][row0] = l0;
           sh.half[half][row0 + 8] = l1;
         }
-        if (tell(3, 0) & 2) break;
+        if (tell(3) & 2) break;
         if (t4 == 0 && half == 0) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -336,121 +360,97 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
       if (lane == 0) raise_status(a.status, DSA_STATUS_WAIT_TIMEOUT);
     }
   } else if (n > 0 && warp == 8) {
-    // ============================ products ============================
-    // Whatever is ready first: the second product of a tile as soon as its P is there (it frees the page), else the
-    // next column group of the first product.  The whole warp runs this loop, its lanes' decisions taken from lane
-    // 0; one lane issues.
-    int qk_i = 0, np = 0, nq = 0, cur_b = -1, pend_n = 0;
-    int pend_stage0 = 0, pend_stage1 = 0, pend_acc0 = 0, pend_acc1 = 0, acc_next = 0;
-    bool q_here = false;
+    // ============================ first products ============================
+    // The whole warp runs this, its lanes' descriptors in uniform registers; one lane issues.
     const uint32_t elected = ptx::elect_one();
     const uint64_t dq = ptx::smem_desc_sw128(q_addr, 16, 1024), dk = ptx::smem_desc_sw128(kv_addr, 16, 1024);
-    const uint64_t dv = ptx::smem_desc_sw128(kv_addr, kTcBlock, 1024), dp = ptx::smem_desc_sw128(p_addr, 16, 1024);
-    auto ready = [&](uint64_t& bar, uint32_t parity) {
-      return __shfl_sync(0xffffffffu, ptx::mbar_test_wait(smem_u32(&bar), parity) ? 1 : 0, 0) != 0;
+    int cur_b = -1, nq = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t& bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(smem_u32(&bar), parity) ? 1 : 0);
     };
-    auto second_product = [&]() {
-      ptx::tc_fence_after();
-      const uint64_t va = dv + (uint32_t)((pend_stage0 * kTcPage) >> 4);
-#pragma unroll
-      for (int c = 0; c < kTcGroups; ++c) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          ptx::mma_bf16_warp(elected, tmem + c * kTcRows, va + ((2 * c * kTcBlock + ks * 2048) >> 4), dp + ((ks * 32) >> 4),
-                             kTcIdescPV, ks == 0 ? pend_acc0 : 1u);
-        if (elected) ptx::tc_commit(smem_u32(&sh.empty[pend_stage0][c]));
+    for (int i = 0; i < n && ok; ++i) {
+      const int s = i & 1, phase = (i >> 1) & 1;
+      wait(sh.full[s][0], phase);
+      if (!ok) break;
+      const TcTile tile = sh.tile[s];
+      if (tile.b != cur_b) {
+        cur_b = tile.b;
+        wait(sh.q_full, nq & 1);
+        ++nq;
       }
-      if (elected) ptx::tc_commit(smem_u32(&sh.p_empty));
+      wait(sh.s_empty[s], phase ^ 1);
+      if (!ok) break;
+      if (tile.live) {
+        const uint32_t d = tmem + kTcSCol + s * 64;
+        const uint64_t ka = dk + (uint32_t)((s * kTcPage) >> 4);
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < kTcGroups; ++g) {
+          if (g > 0) wait(sh.full[s][g], phase);
+#pragma unroll
+          for (int k = 8 * g; k < (g == kTcGroups - 1 ? 36 : 8 * g + 8); ++k)
+            ptx::mma_bf16_warp(elected, d, dq + (((k >> 2) * kTcBlock + (k & 3) * 32) >> 4),
+                               ka + (((k >> 2) * kTcBlock + (k & 3) * 32) >> 4), kTcIdescQK, k ? 1u : 0u);
+        }
+        if (elected) ptx::tc_commit(smem_u32(&sh.s_full[s]));
+      } else if (elected) {
+        ptx::mbar_arrive(smem_u32(&sh.s_full[s]));   // nothing to multiply
+      }
+      if ((tile.last || i == n - 1) && elected) ptx::tc_commit(smem_u32(&sh.q_empty));
       __syncwarp();
-      ++np;
-      pend_stage0 = pend_stage1;
-      pend_acc0 = pend_acc1;
-      --pend_n;
+    }
+    if (!ok && lane == 0) {
+      sh.abort_flag = 1;
+      raise_status(a.status, DSA_STATUS_WAIT_TIMEOUT);
+    }
+    __syncwarp();
+  } else if (n > 0 && warp == 9) {
+    // ============================ second products ============================
+    const uint32_t elected = ptx::elect_one();
+    const uint64_t dv = ptx::smem_desc_sw128(kv_addr, kTcBlock, 1024), dp = ptx::smem_desc_sw128(p_addr, 16, 1024);
+    int cur_b = -1, np = 0;
+    uint32_t acc = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t& bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(smem_u32(&bar), parity) ? 1 : 0);
     };
-    uint64_t idle_since = 0;
-    while (qk_i < n || pend_n > 0) {
-      bool progressed = false;
-      if (pend_n > 0 && ready(sh.p_full, np & 1)) {
-        second_product();
-        progressed = true;
-      } else if (qk_i < n) {
-        const int s = qk_i & 1, phase = (qk_i >> 1) & 1;
-        if (ready(sh.full[s][0], phase) && ready(sh.s_empty[s], phase ^ 1)) {
-          const TcTile tile = sh.tile[s];
-          if (tile.b != cur_b) {
-            cur_b = tile.b;
-            q_here = false;
-            acc_next = 0;                            // the request's first product overwrites O^T
-          }
-          if (!q_here) {
-            q_here = ready(sh.q_full, nq & 1);
-            if (q_here) ++nq;
-          }
-          if (q_here) {
-            bool landed = true;
-            if (tile.live) {
-              const uint32_t d = tmem + kTcSCol + s * 64;
-              const uint64_t ka = dk + (uint32_t)((s * kTcPage) >> 4);
-#pragma unroll
-              for (int g = 0; g < kTcGroups; ++g) {
-                if (g > 0) {
-                  landed = landed && ptx::mbar_wait(smem_u32(&sh.full[s][g]), phase);
-                  __syncwarp();
-                  if (pend_n > 0 && ready(sh.p_full, np & 1)) second_product();
-                }
-                if (g == 0) ptx::tc_fence_after();
-#pragma unroll
-                for (int k = 8 * g; k < (g == kTcGroups - 1 ? 36 : 8 * g + 8); ++k)
-                  ptx::mma_bf16_warp(elected, d, dq + (((k >> 2) * kTcBlock + (k & 3) * 32) >> 4),
-                                     ka + (((k >> 2) * kTcBlock + (k & 3) * 32) >> 4), kTcIdescQK, k ? 1u : 0u);
-              }
-              if (elected) ptx::tc_commit(smem_u32(&sh.s_full[s]));
-              if (pend_n == 0) {
-                pend_stage0 = s;
-                pend_acc0 = acc_next;
-              } else {
-                pend_stage1 = s;
-                pend_acc1 = acc_next;
-              }
-              ++pend_n;
-              acc_next = 1;
-            } else {
-              // nothing to multiply; a group is handed back once the producer is past it, never before
-              for (int c = 1; c < kTcGroups; ++c) landed = landed && ptx::mbar_wait(smem_u32(&sh.full[s][c]), phase);
-              __syncwarp();
-              if (elected) {
-                ptx::mbar_arrive(smem_u32(&sh.s_full[s]));
-                for (int c = 0; c < kTcGroups; ++c) ptx::mbar_arrive(smem_u32(&sh.empty[s][c]));
-              }
-            }
-            if (!__all_sync(0xffffffffu, landed)) {
-              if (lane == 0) {
-                sh.abort_flag = 1;
-                raise_status(a.status, DSA_STATUS_WAIT_TIMEOUT);
-              }
-              break;
-            }
-            if ((tile.last || qk_i == n - 1) && elected) ptx::tc_commit(smem_u32(&sh.q_empty));
-            ++qk_i;
-            __syncwarp();
-            progressed = true;
-          }
-        }
+    for (int i = 0; i < n && ok; ++i) {
+      const int s = i & 1, phase = (i >> 1) & 1;
+      wait(sh.full[s][0], phase);
+      if (!ok) break;
+      const TcTile tile = sh.tile[s];
+      if (tile.b != cur_b) {
+        cur_b = tile.b;
+        acc = 0;                                     // the request's first product overwrites O^T
       }
-      if (progressed) {
-        idle_since = 0;
+      if (tile.live) {
+        wait(sh.p_full, np & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint64_t va = dv + (uint32_t)((s * kTcPage) >> 4);
+#pragma unroll
+        for (int c = 0; c < kTcGroups; ++c) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            ptx::mma_bf16_warp(elected, tmem + c * kTcRows, va + ((2 * c * kTcBlock + ks * 2048) >> 4),
+                               dp + ((ks * 32) >> 4), kTcIdescPV, ks == 0 ? acc : 1u);
+          if (elected) ptx::tc_commit(smem_u32(&sh.empty[s][c]));
+        }
+        if (elected) ptx::tc_commit(smem_u32(&sh.p_empty));
+        ++np;
+        acc = 1;
       } else {
-        const uint64_t now = __shfl_sync(0xffffffffu, ptx::global_timer_ns(), 0);
-        const int stop = __shfl_sync(0xffffffffu, sh.abort_flag, 0);
-        if (idle_since == 0) idle_since = now;
-        if (stop || now - idle_since > 250000000ull) {
-          if (!stop && lane == 0) {
-            sh.abort_flag = 1;
-            raise_status(a.status, DSA_STATUS_WAIT_TIMEOUT);
-          }
-          break;
-        }
+        // nothing to multiply; a group is handed back once the producer is past it, never before
+        for (int c = 1; c < kTcGroups; ++c) wait(sh.full[s][c], phase);
+        if (ok && elected)
+          for (int c = 0; c < kTcGroups; ++c) ptx::mbar_arrive(smem_u32(&sh.empty[s][c]));
       }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) {
+      sh.abort_flag = 1;
+      raise_status(a.status, DSA_STATUS_WAIT_TIMEOUT);
     }
     __syncwarp();
   } else if (n > 0) {
