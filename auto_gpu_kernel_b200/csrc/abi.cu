@@ -527,7 +527,7 @@ int dsa_rotary_append(const void* q_pe, int64_t q_token_stride, int64_t q_head_s
   if (tokens == 0) return DSA_OK;
   if (!q_pe || !ckv || !kpe || !positions || !inv_freq || !slots || !q_out || !ckv_cache || !kpe_cache)
     return DSA_ERR_NULL_POINTER;
-  if (tokens < 0 || heads < 1 || heads > 128 || axes < 1 || axes > 4 || num_slots <= 0 || positions_stride < tokens ||
+  if (tokens < 0 || heads < 1 || heads > 128 || axes < 1 || axes > 4 || num_slots <= 0 || positions_stride < 0 ||
       ckv_stride < dsa::kCkv || kpe_stride < dsa::kKpe || q_token_stride < dsa::kKpe || q_head_stride < dsa::kKpe)
     return DSA_ERR_BAD_SHAPE;
   for (int i = 0; i < dsa::kKpe / 2; ++i)

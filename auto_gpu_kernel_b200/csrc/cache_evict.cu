@@ -7,8 +7,7 @@
 // Two kernels.  The choice is a radix selection over the order-preserving 32-bit keys of the weights (11 + 11 + 10 bits):
 // a cluster of CTAs per request, each with a slice of the row as keys in shared memory, adds its three histograms up
 // through distributed shared memory; then every thread counts what it keeps of a run of its own, one scan gives the
-// places, and the positions are written in order.  It is a chain of sweeps and barriers, so the cluster is as large as
-// the machine allows while a slice stays worth a sweep.  The move is bound by memory: 1152 B (+ 132 B of an index key and
+// places, and the positions are written in order.  The move is bound by memory: 1152 B (+ 132 B of an index key and
 // its scale) in and out per kept token; the kept weights go along with it.
 #include <cooperative_groups.h>
 
@@ -198,11 +197,12 @@ evict_choose_kernel(const EvictArgs a) {
   if (csize > 1) cluster.sync();         // nobody leaves while its counts may be read
 }
 
-// Clusters of this many CTAs can be resident at once (a cluster needs its SMs inside one GPC).
+// CTAs per request: up to four while the SMs hold them at once and a slice stays 8192 keys; less is not worth the
+// cluster's barriers.  Whole call with 512 kept tokens, 1 / 2 / 4 / 8 CTAs: 4 x 8192 tokens 16.4 / 18.1 / 18.5 / 21.3 us,
+// 64 x 16384 38.4 / 34.7 / 47.2 / 106, 16 x 32768 32.9 / 26.7 / 22.6 / 44.3, 32 x 32768 44.8 / 34.5 / 30.7 / 66.4.
 int ev_cluster(int batch, int64_t longest, int sms) {
   int c = 1;
-  // a slice of 2048 keys is two sweeps of a CTA; less is not worth the cluster's barriers
-  while (c < 8 && longest / (2 * c) >= 2048 && (int64_t)batch * 2 * c <= (c == 4 ? sms * 4 / 5 : sms * 9 / 10)) c *= 2;
+  while (c < 4 && longest / (2 * c) >= 8192 && (int64_t)batch * 2 * c <= sms * 9 / 10) c *= 2;
   return c;
 }
 

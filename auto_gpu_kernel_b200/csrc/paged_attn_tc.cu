@@ -9,11 +9,15 @@
 // for M: 512 output columns are four M = 128 blocks, and the accumulator is 256 of the 512 TMEM columns, which
 // leaves room for two S buffers.
 //
-// Bounds: an instruction costs max(45.6, N/2) cycles, so a page is 52 x 45.6 = 2.4 k cycles of the tensor pipe against
-// 3.2 k in which an SM's share of the memory bandwidth delivers it.  q (72 KB) and P leave shared memory for two
-// pages only, so what counts is how long a page stays: every page travels as four column groups with barriers of
-// their own -- the first product follows the groups as they land, the second hands each back as it is done --
-// and the producer asks L2 for the pages that have no place yet.
+// Bounds: an instruction reads its operands from shared memory at 128 B per cycle, so the first product's cost 32 cycles
+// (M = N = 64; measured 36 when a converged warp issues them, 55-160 from a branch of one lane, whose descriptors have
+// to be moved to uniform registers each time) and the second's 48 (49): 2.1 k cycles per page, against the 3.2 k in
+// which an SM's share of the memory bandwidth delivers it.  q (72 KB) and P leave shared memory for two pages only, so
+// what counts is how long a page stays: every page travels as four column groups with barriers of their own -- the
+// first product follows the groups as they land, the second hands each back as it is done -- the two products are
+// issued by warps of their own, and L2 is asked for the pages that have no place yet.  Steady state 3.0 k cycles per
+// page; 16 requests x 8192 tokens x 64 rows take 47 us, floor 23.4 us (memory): 8 us until the first page is there, 22 us
+// of pages, 3 us to store the partial results, the rest the join.
 //
 // Roles (352 threads): warps 0-7 softmax and epilogue, warp 8 issues the first products and warp 9 the second ones (a
 // second product is not to wait behind a first one whose page is still landing), warp 10 the TMA loads.  Every wait is

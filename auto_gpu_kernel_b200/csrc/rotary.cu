@@ -6,7 +6,7 @@
 //
 // Bound by memory (64 * 2 * 2 B per head and token, 2304 B per token for the cache rows).  The angle is a product of up to
 // 31 + 24 bits and is reduced in double precision: in fp32 a position of 10^5 would already be 10^-2 off.  One
-// sine and cosine per pair and token, by the lane of that number; the lanes that rotate get theirs by shuffle.
+// sine and cosine per pair and warp, by the lane of that number; the lanes that rotate get theirs by shuffle.
 #include "common.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -77,8 +77,8 @@ __device__ __forceinline__ void turn_halves(uint4& lo, uint4& hi, const float (&
   }
 }
 
-// One warp per (token, 16 heads); the first group of a token's heads also takes its cache rows.  A 64-wide row is 8
-// chunks of 16 bytes: a lane has one chunk of neighbours, or the chunks c and c + 4 of halves.
+// One warp per (token, 16 heads) and one per token for its cache rows.  A 64-wide row is 8 chunks of 16 bytes: a lane has one
+// chunk of neighbours, or the chunks c and c + 4 of halves.
 template <bool kNeighbours>
 __global__ void __launch_bounds__(kRoThreads)
 rotary_append_kernel(const RotaryArgs a) {
@@ -88,73 +88,73 @@ rotary_append_kernel(const RotaryArgs a) {
   const int64_t unit = (int64_t)blockIdx.x * (kRoThreads / 32) + (threadIdx.x >> 5);
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  if (unit >= (int64_t)a.tokens * a.groups) return;
-  const int t = (int)(unit / a.groups), grp = (int)(unit % a.groups);
+  if (unit >= (int64_t)a.tokens * (a.groups + 1)) return;
+  // units of the heads first, then those of the cache rows
+  const bool cache = unit >= (int64_t)a.tokens * a.groups;
+  const int64_t first = cache ? unit - (int64_t)a.tokens * a.groups : unit;
+  const int t = (int)(cache ? first : first / a.groups), grp = (int)(cache ? 0 : first % a.groups);
   const int c = lane % kLanes, sub = lane / kLanes;
-
-  // all loads first
-  uint4 x[kRounds], y[kRounds];
-  const uint4* q = a.q + (int64_t)t * a.q_token;
+  float cs[kPairs], sn[kPairs];
+  auto turns = [&]() {
+    const int axis = (int)((a.pair_axes >> (2 * lane)) & 3u);
+    // in half turns: the remainder of a whole number of turns is exact in double
+    const double half = (double)__ldg(a.positions + axis * a.positions_stride + t) *
+                        ((double)__ldg(a.inv_freq + lane) * 0.31830988618379067154);
+    float co, si;
+    sincospif((float)(half - 2.0 * rint(0.5 * half)), &si, &co);
+    spread<kPairs>(co, si, kPairs * c, cs, sn);
+  };
+  if (!cache) {
+    uint4 x[kRounds], y[kRounds];                  // all loads first
+    const uint4* q = a.q + (int64_t)t * a.q_token;
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) {
-    const int h = grp * kRoHeads + k * kAtOnce + sub;
-    if (h < a.heads) {
-      x[k] = q[(int64_t)h * a.q_head + c];
-      if (!kNeighbours) y[k] = q[(int64_t)h * a.q_head + c + 4];
-    }
-  }
-  int64_t slot = -1;
-  uint4 r0, r1, kx, ky;
-  if (grp == 0) {
-    const int v = __ldg(a.slots + t);
-    if (v >= a.num_slots) {
-      if (lane == 0) raise_status(a.status, DSA_STATUS_BAD_SLOT);
-    } else {
-      slot = v;
-    }
-    if (slot >= 0) {
-      r0 = a.ckv[(int64_t)t * a.ckv_stride + lane];
-      r1 = a.ckv[(int64_t)t * a.ckv_stride + lane + 32];
-      if (sub == 0) {
-        kx = a.kpe[(int64_t)t * a.kpe_stride + c];
-        if (!kNeighbours) ky = a.kpe[(int64_t)t * a.kpe_stride + c + 4];
+    for (int k = 0; k < kRounds; ++k) {
+      const int h = grp * kRoHeads + k * kAtOnce + sub;
+      if (h < a.heads) {
+        x[k] = q[(int64_t)h * a.q_head + c];
+        if (!kNeighbours) y[k] = q[(int64_t)h * a.q_head + c + 4];
       }
     }
-  }
-  const int axis = (int)((a.pair_axes >> (2 * lane)) & 3u);
-  const double angle = (double)__ldg(a.positions + axis * a.positions_stride + t) * (double)__ldg(a.inv_freq + lane);
-  constexpr double kTurn = 6.283185307179586476925287;
-  const float rem = (float)fma(-rint(angle * (1.0 / kTurn)), kTurn, angle);
-  float co, si, cs[kPairs], sn[kPairs];
-  sincosf(rem, &si, &co);
-  spread<kPairs>(co, si, kPairs * c, cs, sn);
-
-  uint4* out = a.q_out + (int64_t)t * a.heads * 8;
+    turns();
+    uint4* out = a.q_out + (int64_t)t * a.heads * 8;
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) {
-    const int h = grp * kRoHeads + k * kAtOnce + sub;
-    if (h >= a.heads) continue;
-    if constexpr (kNeighbours) {
-      out[h * 8 + c] = turn_neighbours(x[k], cs, sn);
-    } else {
-      turn_halves(x[k], y[k], cs, sn);
-      out[h * 8 + c] = x[k];
-      out[h * 8 + c + 4] = y[k];
-    }
-  }
-  if (slot >= 0) {
-    uint4* row = a.ckv_cache + slot * (kCkv * 2 / 16);
-    row[lane] = r0;
-    row[lane + 32] = r1;
-    if (sub == 0) {
-      uint4* key = a.kpe_cache + slot * 8;
+    for (int k = 0; k < kRounds; ++k) {
+      const int h = grp * kRoHeads + k * kAtOnce + sub;
+      if (h >= a.heads) continue;
       if constexpr (kNeighbours) {
-        key[c] = turn_neighbours(kx, cs, sn);
+        out[h * 8 + c] = turn_neighbours(x[k], cs, sn);
       } else {
-        turn_halves(kx, ky, cs, sn);
-        key[c] = kx;
-        key[c + 4] = ky;
+        turn_halves(x[k], y[k], cs, sn);
+        out[h * 8 + c] = x[k];
+        out[h * 8 + c + 4] = y[k];
       }
+    }
+    return;
+  }
+  const int slot = __ldg(a.slots + t);
+  if (slot < 0) return;
+  if (slot >= a.num_slots) {
+    if (lane == 0) raise_status(a.status, DSA_STATUS_BAD_SLOT);
+    return;
+  }
+  const uint4 r0 = a.ckv[(int64_t)t * a.ckv_stride + lane], r1 = a.ckv[(int64_t)t * a.ckv_stride + lane + 32];
+  uint4 kx = make_uint4(0, 0, 0, 0), ky = kx;
+  if (sub == 0) {
+    kx = a.kpe[(int64_t)t * a.kpe_stride + c];
+    if (!kNeighbours) ky = a.kpe[(int64_t)t * a.kpe_stride + c + 4];
+  }
+  turns();
+  uint4* row = a.ckv_cache + (int64_t)slot * (kCkv * 2 / 16);
+  row[lane] = r0;
+  row[lane + 32] = r1;
+  if (sub == 0) {
+    uint4* key = a.kpe_cache + (int64_t)slot * 8;
+    if constexpr (kNeighbours) {
+      key[c] = turn_neighbours(kx, cs, sn);
+    } else {
+      turn_halves(kx, ky, cs, sn);
+      key[c] = kx;
+      key[c + 4] = ky;
     }
   }
 }
@@ -170,7 +170,7 @@ cudaError_t launch_rotary_append(const void* q, int64_t q_token, int64_t q_head,
                   static_cast<const uint4*>(kpe), kpe_stride / 8, positions, positions_stride, inv_freq, pair_axes, slots,
                   static_cast<uint4*>(q_out), static_cast<uint4*>(ckv_cache), static_cast<uint4*>(kpe_cache), status, num_slots,
                   tokens, heads, (heads + kRoHeads - 1) / kRoHeads};
-  const int64_t units = (int64_t)tokens * a.groups;
+  const int64_t units = (int64_t)tokens * (a.groups + 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((units + kRoThreads / 32 - 1) / (kRoThreads / 32)));
   cfg.blockDim = dim3(kRoThreads);

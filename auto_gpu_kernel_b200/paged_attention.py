@@ -110,7 +110,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
-    its request; other entries stay as they were."""
+    its request; other entries stay as they were.  The call's scratch then holds the logits, 256 bytes per query row
+    and page of the table, so a table much wider than its lengths costs memory."""
     shape, index = q_nope.shape, q_nope.get_device()
     bf16 = torch.bfloat16
     if not (index >= 0 and len(shape) == 3 and shape[2] == CKV and 1 <= shape[1] <= MAX_HEADS
@@ -124,6 +125,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     batch, max_pages = block_table.shape
     if rows == 0:
         return None
+    if abs(output.data_ptr() - q_nope.data_ptr()) < 2 * CKV * rows * heads:
+        raise ValueError("paged attention: output must not overlap q_nope")
     if batch == 0 or rows % batch:
         raise ValueError(f"paged attention: {rows} query tokens are no multiple of the {batch} requests")
     old = new = old_stride = new_stride = 0
@@ -148,7 +151,7 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     scratch = torch.empty(need, dtype=torch.uint8, device=q_nope.device)
     rc = workspace.call_on(
         index, lib.dsa_paged_attn, q_nope.data_ptr(), q_pe.data_ptr(), ckv_cache.data_ptr(), kpe_cache.data_ptr(),
-        seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), sm_scale, output.data_ptr(), lse.data_ptr(), old,
+        seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), float(sm_scale), output.data_ptr(), lse.data_ptr(), old,
         old_stride, new, new_stride, batch, tokens, heads, ckv_cache.shape[0], max_pages, scratch.data_ptr(), need)
     if rc:
         _lib.check(rc, "dsa_paged_attn")

@@ -25,14 +25,14 @@ def sections(*counts):
 
 @functools.lru_cache(maxsize=64)
 def _pack(pair_axes, axes):
-    """The axis of every pair in two bits."""
+    """The axes (a byte per pair) in two bits each."""
     if len(pair_axes) != PAIRS:
         raise ValueError(f"rotary: pair_axes must have {PAIRS} entries")
     packed = 0
     for i, axis in enumerate(pair_axes):
-        if not 0 <= axis < axes:
+        if axis >= axes:
             raise ValueError(f"rotary: pair {i} asks for axis {axis} of {axes}")
-        packed |= int(axis) << (2 * i)
+        packed |= axis << (2 * i)
     return packed
 
 
@@ -42,7 +42,8 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
     with `ckv` [n,512] at global slot `slots[t]` of the paged caches [P,64,512] / [P,64,64] (-1 skips the token's
     cache rows; two equal slots race).
 
-    Pair i of token t turns by positions[pair_axes[i], t] * inv_freq[i]: `positions` [axes,n] int32 with one to four axes,
+    Pair i of token t turns by positions[pair_axes[i], t] * inv_freq[i]: `positions` [axes,n] int32 with one to four axes
+    (rows may be expanded),
     `inv_freq` [32] float32, `pair_axes` 32 axis numbers (see `sections`).  A pair is (2i, 2i+1) when `interleaved`,
     else (i, i+32)."""
     if not q_pe.is_cuda:
@@ -63,7 +64,9 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
     if inv_freq.dim() != 1 or inv_freq.shape[0] != PAIRS or inv_freq.dtype is not torch.float32 \
             or not inv_freq.is_contiguous():
         raise ValueError("rotary: inv_freq must be a contiguous [32] float32 tensor")
-    packed = _pack(tuple(pair_axes), axes)
+    if isinstance(pair_axes, int):
+        raise ValueError(f"rotary: pair_axes must be {PAIRS} axis numbers")
+    packed = _pack(bytes(pair_axes), axes)
     if slots.dim() != 1 or slots.shape[0] != n or slots.dtype is not i32 or not slots.is_contiguous():
         raise ValueError("rotary: slots must be a contiguous [n] int32 tensor")
     if ckv_cache.shape[-1] != 512 or kpe_cache.shape[-1] != 64 or not ckv_cache.is_contiguous() \

@@ -199,7 +199,7 @@ int dsa_kv_cache_append(const void* ckv, int64_t ckv_stride, const void* kpe, in
  *   ckv     [num_pages,64,512] bf16      kpe  [num_pages,64,64] bf16
  *   seq_lens [batch] int32 cached tokens, the new ones among them; block_table [batch,max_pages] int32, row stride
  *           `block_table_stride` elements (0 = every request shares one row)
- *   out     [batch*tokens_per_request,heads,512] bf16   lse [..,heads] fp32 (base-2 log-sum-exp)
+ *   out     [batch*tokens_per_request,heads,512] bf16 (not over q_nope)   lse [..,heads] fp32 (base-2 log-sum-exp)
  * Token i of a request's n new ones stands at position seq_len - n + i and sees the positions up to its own; one
  * that stands before the request's beginning sees nothing and gets out = 0 and lse = -inf.  Positions at or
  * behind seq_len may hold anything; those in front of it must be finite.  seq_len is taken within
@@ -253,7 +253,7 @@ int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, co
  *   angle[t,i] = positions[axis of pair i, t] * inv_freq[i], in 64 bits; axis of pair i = bits 2i, 2i+1 of `pair_axes`
  *   q_pe  [tokens,heads,64] bf16, token and head strides in elements (multiples of 8)
  *   ckv [tokens,512], kpe [tokens,64] bf16, row strides in elements (multiples of 8)
- *   positions [axes,tokens] int32, row stride in elements; inv_freq [32] fp32
+ *   positions [axes,tokens] int32, row stride in elements (0 = one row for every axis); inv_freq [32] fp32
  *   interleaved 1: the pairs are the neighbours (2i, 2i+1); 0: (i, i + 32)
  *   q_out [tokens,heads,64] bf16 contiguous (may be q_pe where that is contiguous) receives the rotated queries of
  *   every token; ckv_cache / kpe_cache [num_slots,512 / 64] receive ckv[t] and the rotated kpe[t] at slot slots[t]

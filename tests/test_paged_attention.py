@@ -270,6 +270,34 @@ def test_other_stream_and_two_at_once():
 
 
 @pytest.mark.gpu
+def test_several_calls_in_a_row_on_changing_shapes():
+    """Calls whose scratch buffers take one another's place, without a synchronisation in between."""
+    from auto_gpu_kernel_b200 import paged_attention
+    cases = [make([9000, 5], seed=30), make([700, 3, 0, 64], heads=64, seed=31), make([40], tokens=3, seed=32),
+             make([20000], heads=20, seed=33), make([130] * 200, seed=34)]
+    want = []
+    for c in cases:
+        want.append(paged_attention.run(*c, SCALE))
+        torch.cuda.synchronize()
+    got = [[paged_attention.run(*c, SCALE) for c in cases] for _ in range(8)]
+    torch.cuda.synchronize()
+    for round_ in got:
+        for x, y in zip(round_, want):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+@pytest.mark.gpu
+def test_on_a_device_that_is_not_current():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    from auto_gpu_kernel_b200 import paged_attention
+    args = make([900, 70], seed=35)
+    want = paged_attention.run(*args, SCALE)
+    there = paged_attention.run(*[t.to("cuda:1") for t in args], SCALE)
+    assert torch.equal(want[0].cpu(), there[0].cpu()) and torch.equal(want[1].cpu(), there[1].cpu())
+
+
+@pytest.mark.gpu
 def test_captured_graphs_keep_their_own_workspaces():
     from auto_gpu_kernel_b200 import paged_attention
     cases = [make([3000, 10], seed=16), make([9000, 900, 64], seed=17)]
@@ -335,6 +363,9 @@ def test_refusals():
     big = torch.zeros(4, 128, device="cuda")
     refuses(ValueError, token_weights=big[:2], new_token_weights=big[1:3])
     refuses(RuntimeError, new_token_weights=w.cpu())
+    refuses(ValueError, output=args[0])
+    flat = torch.zeros(args[0].numel() + 512, dtype=torch.bfloat16, device="cuda")
+    refuses(ValueError, a0=flat[:args[0].numel()].view(args[0].shape), output=flat[512:].view(args[0].shape))
     empty = paged_attention.run(args[0][:0], args[1][:0], *args[2:4], args[4][:0], args[5][:0], SCALE)
     assert empty[0].shape == (0, 16, 512)
     none = paged_attention.run(*args[:5], args[5][:, :0], SCALE)

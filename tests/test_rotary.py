@@ -68,7 +68,7 @@ def test_host_side_argument_errors():
     assert call(n=0, q=None) == 0
     for name in ("q", "c", "k", "p", "f", "s", "o", "cc", "kc"):
         assert call(**{name: None}) == -1, name
-    for kw in (dict(n=-1), dict(h=0), dict(h=129), dict(axes=0), dict(axes=5), dict(slots=0), dict(ps=3), dict(cs=511), dict(ks=63),
+    for kw in (dict(n=-1), dict(h=0), dict(h=129), dict(axes=0), dict(axes=5), dict(slots=0), dict(ps=-1), dict(cs=511), dict(ks=63),
                dict(qt=63), dict(qh=63), dict(pa=2), dict(pa=3 << 62), dict(axes=1)):
         assert call(**kw) == -2, kw
     for kw in (dict(qt=1028), dict(qh=68), dict(cs=516), dict(ks=68), dict(q=8), dict(c=8), dict(k=8), dict(o=8), dict(cc=8),
@@ -118,6 +118,15 @@ def test_skipped_strided_and_in_place():
     plain["q_pe"] = q
     assert rotary.append(**plain, q_out=q) is q
     assert torch.equal(first, q)
+
+
+@pytest.mark.gpu
+def test_expanded_positions():
+    case = make(50, axes=1, seed=8)
+    want = rotary.append(**case, interleaved=True)
+    case["positions"] = case["positions"].expand(4, -1)          # text: every axis at the same position
+    case["pair_axes"] = rotary.sections(8, 8, 8, 8)
+    assert torch.equal(check(case, True, "expanded"), want)
 
 
 @pytest.mark.gpu
@@ -184,6 +193,8 @@ def test_refusals():
     refuses(ValueError, inv_freq=case["inv_freq"][:31])
     refuses(ValueError, pair_axes=[0] * 31)
     refuses(ValueError, pair_axes=[0] * 31 + [-1])
+    refuses(ValueError, pair_axes=32)
+    refuses(ValueError, pair_axes=[0] * 31 + [300])
     refuses(ValueError, slots=case["slots"].long())
     refuses(ValueError, kpe_cache=case["kpe_cache"][:1])
     refuses(ValueError, q_out=q[:, :, :32])
