@@ -69,7 +69,7 @@ def rows_of(what, name, t, batch, width, dtype, index):
     return t.data_ptr(), max(t.stride(0), t.shape[1])
 
 
-def _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, lse):
+def _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table):
     what = "paged attention"
     if not q_nope.is_cuda:
         raise RuntimeError(f"{what}: CUDA tensors required (this operator has no CPU path)")
@@ -85,12 +85,16 @@ def _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, l
         raise ValueError(f"{what}: 1 to {MAX_HEADS} heads, got {heads}")
     if q_pe.shape != (rows, heads, KPE) or q_pe.dtype != torch.bfloat16:
         raise ValueError(f"{what}: q_pe must be [B*n,heads,64] bf16")
-    if output.shape != q_nope.shape or output.dtype != torch.bfloat16 or lse.shape != (rows, heads) \
-            or lse.dtype != torch.float32:
-        raise ValueError(f"{what}: output must be [B*n,heads,512] bf16 and lse [B*n,heads] float32")
-    if not (q_nope.is_contiguous() and q_pe.is_contiguous() and output.is_contiguous() and lse.is_contiguous()):
-        raise ValueError(f"{what}: q_nope, q_pe, output and lse must be contiguous")
-    raise RuntimeError(f"{what}: all tensors must be on cuda:{index}")
+    if not (q_nope.is_contiguous() and q_pe.is_contiguous()):
+        raise ValueError(f"{what}: q_nope and q_pe must be contiguous")
+    raise RuntimeError(f"{what}: q_pe must be on cuda:{index}")
+
+
+def _check_output(name, t, shape, dtype, index):
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+        raise ValueError(f"paged attention: {name} must be a contiguous {list(shape)} {dtype} tensor")
+    if t.get_device() != index:
+        raise RuntimeError(f"paged attention: {name} must be on cuda:{index}")
 
 
 @functools.lru_cache(maxsize=512)
@@ -99,34 +103,29 @@ def _workspace_bytes(index, batch, tokens, heads, max_pages, with_weights):
         return _lib.load().dsa_paged_attn_workspace_bytes(batch, tokens, heads, max_pages, with_weights)
 
 
-def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights=None,
-           new_token_weights=None):
-    """Write the attention output and the base-2 LSE in place; enqueued on the current stream, returns None.
-
-    q_nope [B*n,heads,512] / q_pe [B*n,heads,64] bf16: the n newest tokens of every request, oldest first (1 to 128
-    heads).  `seq_lens` counts the cached tokens of each request, the new ones among them: token i of n sees the
-    positions below seq_len - n + 1 + i, and one that sees none gets output 0 and lse -inf.  Cache rows at or
-    behind seq_len may hold anything, those in front of it must be finite.
-
-    `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
-    shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
-    its request; other entries stay as they were.  The call's scratch then holds the logits, 256 bytes per query row
-    and page of the table, so a table much wider than its lengths costs memory."""
+def _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights,
+            new_token_weights):
     shape, index = q_nope.shape, q_nope.get_device()
     bf16 = torch.bfloat16
     if not (index >= 0 and len(shape) == 3 and shape[2] == CKV and 1 <= shape[1] <= MAX_HEADS
-            and q_pe.shape == (shape[0], shape[1], KPE) and output.shape == shape and lse.shape == shape[:2]
-            and q_nope.dtype is bf16 and q_pe.dtype is bf16 and output.dtype is bf16 and lse.dtype is torch.float32
-            and q_nope.is_contiguous() and q_pe.is_contiguous() and output.is_contiguous() and lse.is_contiguous()
-            and q_pe.get_device() == index and output.get_device() == index and lse.get_device() == index
+            and q_pe.shape == (shape[0], shape[1], KPE) and q_nope.dtype is bf16 and q_pe.dtype is bf16
+            and q_nope.is_contiguous() and q_pe.is_contiguous() and q_pe.get_device() == index
             and tables_ok(seq_lens, block_table, index) and caches_ok(ckv_cache, kpe_cache, index)):
-        _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, output, lse)
+        _refuse(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table)
+    if output is None:
+        output = q_nope.new_empty((shape[0], shape[1], CKV))
+    else:
+        _check_output("output", output, shape, bf16, index)
+        if abs(output.data_ptr() - q_nope.data_ptr()) < 2 * q_nope.numel():
+            raise ValueError("paged attention: output must not overlap q_nope")
+    if lse is None:
+        lse = q_nope.new_empty((shape[0], shape[1]), dtype=torch.float32)
+    else:
+        _check_output("lse", lse, shape[:2], torch.float32, index)
     rows, heads, _ = shape
     batch, max_pages = block_table.shape
     if rows == 0:
-        return None
-    if abs(output.data_ptr() - q_nope.data_ptr()) < 2 * CKV * rows * heads:
-        raise ValueError("paged attention: output must not overlap q_nope")
+        return output, lse
     if batch == 0 or rows % batch:
         raise ValueError(f"paged attention: {rows} query tokens are no multiple of the {batch} requests")
     old = new = old_stride = new_stride = 0
@@ -143,7 +142,7 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     if max_pages == 0:
         output.zero_()
         lse.fill_(float("-inf"))
-        return None
+        return output, lse
     lib = _lib.load()
     tokens = rows // batch
     need = _workspace_bytes(index, batch, tokens, heads, max_pages, 1 if new else 0)
@@ -155,16 +154,29 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
         old_stride, new, new_stride, batch, tokens, heads, ckv_cache.shape[0], max_pages, scratch.data_ptr(), need)
     if rc:
         _lib.check(rc, "dsa_paged_attn")
-    return None
+    return output, lse
+
+
+def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights=None,
+           new_token_weights=None):
+    """Write the attention output and the base-2 LSE in place; enqueued on the current stream, returns None.
+
+    q_nope [B*n,heads,512] / q_pe [B*n,heads,64] bf16: the n newest tokens of every request, oldest first (1 to 128
+    heads).  `seq_lens` counts the cached tokens of each request, the new ones among them: token i of n sees the
+    positions below seq_len - n + 1 + i, and one that sees none gets output 0 and lse -inf.  Cache rows at or
+    behind seq_len may hold anything, those in front of it must be finite.
+
+    `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
+    shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
+    its request; other entries stay as they were.  The call's scratch then holds the logits, 256 bytes per query row
+    and page of the table, so a table much wider than its lengths costs memory."""
+    if output is None or lse is None:
+        raise ValueError("paged attention: kernel() needs output and lse")
+    _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights, new_token_weights)
 
 
 def run(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output=None, lse=None, token_weights=None,
         new_token_weights=None):
     """Value-returning form: allocates the outputs that are not passed; returns (output, lse)."""
-    if output is None:
-        output = q_nope.new_empty(tuple(q_nope.shape))
-    if lse is None:
-        lse = q_nope.new_empty(tuple(q_nope.shape[:-1]), dtype=torch.float32)
-    kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights,
-           new_token_weights)
-    return output, lse
+    return _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights,
+                   new_token_weights)
