@@ -6,6 +6,9 @@
     python -m auto_gpu_kernel_b200.run_case attention --batch 64 --context 8192 --variant 0
     python -m auto_gpu_kernel_b200.run_case block     --batch 64 --context 32768
     python -m auto_gpu_kernel_b200.run_case prefill   --batch 4096 --context 16384
+    python -m auto_gpu_kernel_b200.run_case paged     --batch 64 --context 32768 [--heads 128] [--new-tokens 4] [--weights]
+    python -m auto_gpu_kernel_b200.run_case evict     --batch 32 --context 32768 --budget 8192
+    python -m auto_gpu_kernel_b200.run_case rotary    --batch 16384
     python -m auto_gpu_kernel_b200.run_case mma-rate         (issue cost of tcgen05.mma / mma.sync shapes)
 
 Meant for profilers (the launches of one kernel in a small process) and for quick A/B timing.
@@ -60,7 +63,8 @@ def mma_rate(dev) -> int:
 
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("case", choices=["scorer", "select", "indexer", "attention", "block", "prefill", "mma-rate"])
+    ap.add_argument("case", choices=["scorer", "select", "indexer", "attention", "block", "prefill", "paged",
+                                     "evict", "rotary", "mma-rate"])
     ap.add_argument("--batch", type=int, default=64, help="requests (= query tokens)")
     ap.add_argument("--context", type=int, default=32768, help="tokens per request")
     ap.add_argument("--iters", type=int, default=20)
@@ -68,6 +72,10 @@ def main(argv=None) -> int:
     ap.add_argument("--variant", type=int, default=0,
                     help="scorer/prefill: 0 tcgen05, 1 CUDA-core, 2 streaming tcgen05 kernel; "
                          "attention: 0 mma.sync, 1 CUDA-core, 2 tcgen05")
+    ap.add_argument("--heads", type=int, default=16, help="paged, rotary: query heads")
+    ap.add_argument("--new-tokens", type=int, default=1, help="paged: query tokens per request")
+    ap.add_argument("--weights", action="store_true", help="paged: accumulate every cached token's attention weight")
+    ap.add_argument("--budget", type=int, default=2048, help="evict: tokens kept per request")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--no-pdl", action="store_true")
     args = ap.parse_args(argv)
@@ -114,6 +122,41 @@ def main(argv=None) -> int:
         lse = torch.empty(inp.q_nope.shape[:2], dtype=torch.float32, device=dev)
         fn = lambda: sparse_attention.kernel(*inp.args(), out, lse, variant=args.variant)
         moved = int((inp.sparse_indices >= 0).sum()) * 1152
+    elif args.case in ("paged", "evict"):
+        from . import cache_evict, paged_attention
+        fresh = -(-args.budget // 64) if args.case == "evict" else 0
+        idx = wl.make_indexer_inputs(lens, seed=args.seed, device=dev, extra_pages=args.batch * fresh)
+        pages, width = idx.k_index_cache_fp8.shape[0], idx.block_table.shape[1] * 64
+        gen = torch.Generator(device=dev).manual_seed(args.seed)
+        half = lambda *s: torch.randn(*s, generator=gen, device=dev, dtype=torch.bfloat16)
+        ckv, kpe = half(pages, 64, 512), half(pages, 64, 64)
+        held = torch.rand(args.batch, width, generator=gen, device=dev)
+        if args.case == "paged":
+            rows = args.batch * args.new_tokens
+            a = (half(rows, args.heads, 512), half(rows, args.heads, 64), ckv, kpe, idx.seq_lens, idx.block_table,
+                 192.0 ** -0.5)
+            w = dict(token_weights=held, new_token_weights=held) if args.weights else {}
+            fn = lambda: paged_attention.run(*a, **w)
+            moved = sum(lens) * 1152
+        else:
+            used = torch.zeros(pages, dtype=torch.bool)
+            used[idx.block_table.cpu().long().flatten()] = True
+            free = (~used).nonzero().flatten().to(torch.int32)[:args.batch * fresh].view(args.batch, fresh).to(dev)
+            fn = lambda: cache_evict.run(held, idx.seq_lens, idx.block_table, free, args.budget, ckv, kpe,
+                                         idx.k_index_cache_fp8, keep_first=min(4, args.budget // 2),
+                                         keep_last=min(64, args.budget // 2))
+            moved = 2 * args.batch * min(args.context, args.budget) * (1152 + 132)
+    elif args.case == "rotary":
+        from . import rotary
+        gen = torch.Generator(device=dev).manual_seed(args.seed)
+        half = lambda *s: torch.randn(*s, generator=gen, device=dev, dtype=torch.bfloat16)
+        n, pages = args.batch, -(-args.batch // 64)
+        a = (half(n, args.heads, 64), half(n, 512), half(n, 64),
+             torch.arange(n, dtype=torch.int32, device=dev).expand(3, -1),
+             10000.0 ** (-torch.arange(32, device=dev, dtype=torch.float32) / 32), rotary.sections(16, 8, 8),
+             torch.randperm(pages * 64, generator=gen, device=dev)[:n].to(torch.int32), half(pages, 64, 512), half(pages, 64, 64))
+        fn = lambda: rotary.append(*a)
+        moved = n * (2 * args.heads * 128 + 2 * 1152)
     else:
         blk = wl.make_decode_block_inputs(lens, seed=args.seed, device=dev)
         a = blk.indexer.args()
