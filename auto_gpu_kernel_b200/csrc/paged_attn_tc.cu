@@ -4,10 +4,10 @@
 // 64 query rows of a request per CTA.  A 64-token page is read once from memory for all of them:
 //   S[64 rows, 64 tokens]  = Q[64,576] . K^T      A = q, K-major, resident; B = the page, K-major      (36 tcgen05.mma)
 //   O^T[512, 64 rows]     += V^T[512,64] . P^T    A = the SAME page read MN-major; B = P, K-major       (16 tcgen05.mma)
-// The first product is taken row by row so that a softmax thread has one row and its 64 tokens: maximum and sum need
-// no exchange, and the row of P is eight 16-byte stores.  The second is transposed because the rows are too few
-// for M: 512 output columns are four M = 128 blocks, and the accumulator is 256 of the 512 TMEM columns, which
-// leaves room for two S buffers.
+// The first product has the rows as M: a softmax warp then holds 16 rows x 32 tokens in the fragment order of the warp-level
+// products, and writes P as that order's 4-byte pairs without bank conflicts.  The second is transposed because the
+// rows are too few for M: 512 output columns are four M = 128 blocks, and the accumulator is 256 of the 512 TMEM
+// columns, which leaves room for two S buffers.
 //
 // Bounds: an instruction reads its operands from shared memory at 128 B per cycle, so the first product's cost 32 cycles
 // (M = N = 64; measured 36 when a converged warp issues them, 55-160 from a branch of one lane, whose descriptors have
