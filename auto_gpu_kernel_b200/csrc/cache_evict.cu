@@ -21,8 +21,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kEvThreads = 1024;
+constexpr int kEvThreads = 512;
 constexpr int kEvBins = 2048;
+constexpr int kEvMine = kEvBins / kEvThreads;
+static_assert(kEvMine == 4, "one 16-byte read per thread and histogram");
 constexpr int kEvStaged = 40960;      // keys of a slice that fit in shared memory; longer slices are read again
 
 struct EvictArgs {
@@ -46,7 +48,7 @@ struct EvictArgs {
 };
 
 __device__ __forceinline__ int ev_len(const EvictArgs& a, int b) {
-  const int n = __ldg(a.seq_lens + b);
+  const int n = __ldcg(a.seq_lens + b);
   const int64_t most = (int64_t)a.max_pages * kPage;
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
@@ -67,28 +69,23 @@ __device__ __forceinline__ T ev_scan(T v, T* sums, T& total) {
   }
   if (lane == 31) sums[w] = upto;
   __syncthreads();
-  if (w == 0) {
-    T s = sums[lane];
+  T front = 0;
+  total = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const T u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    sums[lane] = s;
+  for (int i = 0; i < kEvThreads / 32; ++i) {
+    const T u = sums[i];
+    if (i < w) front += u;
+    total += u;
   }
-  __syncthreads();
-  total = sums[31];
-  const T r = (w ? sums[w - 1] : T(0)) + upto - v;
-  __syncthreads();
-  return r;
+  return front + upto - v;
 }
 
 __global__ void __launch_bounds__(kEvThreads)
 evict_choose_kernel(const EvictArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ uint32_t hist[2][kEvBins];
-  __shared__ uint32_t sums[32];
-  __shared__ uint64_t sums64[32];
+  __shared__ alignas(16) uint32_t hist[2][kEvBins];
+  __shared__ uint32_t sums[3][kEvThreads / 32];
+  __shared__ uint64_t sums64[kEvThreads / 32];
   __shared__ uint32_t pick[2];
   __shared__ uint64_t slice_counts;         // of this CTA's slice: above the threshold, and (high half) equal to it
   cg::cluster_group cluster = cg::this_cluster();
@@ -150,27 +147,31 @@ evict_choose_kernel(const EvictArgs a) {
     }
     if (csize > 1) cluster.sync();
     else __syncthreads();
-    // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, of all slices
-    uint32_t c0 = h[kEvBins - 1 - 2 * tid], c1 = h[kEvBins - 2 - 2 * tid];
+    // bins from the top, of all slices: thread t has the kEvMine below 2048 - kEvMine t
+    uint32_t c[kEvMine];
+    const int top = kEvBins - kEvMine * tid;
     for (int r = 0; r < csize; ++r) {
-      if (r == rank) continue;
-      const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(h, r) + kEvBins - 2 - 2 * tid);
-      c0 += v.y;
-      c1 += v.x;
+      const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(h, r) + top - kEvMine);
+      if (r == 0) c[0] = c[1] = c[2] = c[3] = 0;
+      c[0] += v.w;
+      c[1] += v.z;
+      c[2] += v.y;
+      c[3] += v.x;
     }
     uint32_t all;
-    const uint32_t above = ev_scan(c0 + c1, sums, all);
-    if (above < rest && above + c0 >= rest) {
-      pick[0] = kEvBins - 1 - 2 * tid;
-      pick[1] = rest - above;
-    } else if (above + c0 < rest && above + c0 + c1 >= rest) {
-      pick[0] = kEvBins - 2 - 2 * tid;
-      pick[1] = rest - above - c0;
+    uint32_t above = ev_scan(c[0] + c[1] + c[2] + c[3], sums[pass], all);
+#pragma unroll
+    for (int k = 0; k < kEvMine; ++k) {
+      if (above < rest && above + c[k] >= rest) {
+        pick[0] = top - 1 - k;
+        pick[1] = rest - above;
+      }
+      above += c[k];
     }
     __syncthreads();
     prefix = (prefix << bits) | pick[0];
     rest = pick[1];
-    __syncthreads();
+    __syncthreads();                     // before the next pass picks
   }
   // ---- keys above `prefix` are kept, and the first `rest` that equal it ----
   // thread t has the run [t * run, (t + 1) * run) of the slice; an odd run keeps the banks apart
@@ -197,12 +198,13 @@ evict_choose_kernel(const EvictArgs a) {
   if (csize > 1) cluster.sync();         // nobody leaves while its counts may be read
 }
 
-// CTAs per request: up to four while the SMs hold them at once and a slice stays 8192 keys; less is not worth the
-// cluster's barriers.  Whole call with 512 kept tokens, 1 / 2 / 4 / 8 CTAs: 4 x 8192 tokens 16.4 / 18.1 / 18.5 / 21.3 us,
-// 64 x 16384 38.4 / 34.7 / 47.2 / 106, 16 x 32768 32.9 / 26.7 / 22.6 / 44.3, 32 x 32768 44.8 / 34.5 / 30.7 / 66.4.
+// CTAs per request: up to four while the SMs hold them at once and a slice stays 4096 keys; less is not worth the
+// cluster's barriers.  Whole call with 512 or 1024 kept tokens, 1 / 2 / 4 CTAs: 1 x 4096 tokens 12.3 / 14.3 / 14.4 us,
+// 4 x 8192 16.4 / 14.9 / 16.4, 64 x 16384 36.4 / 32.3 / 34.9, 128 x 8192 42.1 / 44.4 / 60.1, 16 x 32768 32.8 / 24.6 / 21.1,
+// 32 x 32768 39.9 / 30.7 / 26.7 (eight were slower throughout).
 int ev_cluster(int batch, int64_t longest, int sms) {
   int c = 1;
-  while (c < 4 && longest / (2 * c) >= 8192 && (int64_t)batch * 2 * c <= sms * 9 / 10) c *= 2;
+  while (c < 4 && longest / (2 * c) >= 4096 && (int64_t)batch * 2 * c <= sms * 9 / 10) c *= 2;
   return c;
 }
 

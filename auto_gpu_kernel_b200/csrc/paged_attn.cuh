@@ -62,14 +62,16 @@ __device__ __forceinline__ float* paged_part(const PagedArgs& a, int block_rows,
 }
 
 // Sum of all requests' tiles, and the tiles in front of this thread's share of the requests (requests
-// [lo, hi) of equal contiguous shares).  By all threads of the CTA; `sums` has one entry per warp.
-template <int kThreads>
+// [lo, hi) of equal contiguous shares).  By all threads of the CTA; `sums` has one entry per warp.  kEarly: in front of the
+// dependency wait, past L1.
+template <int kThreads, bool kEarly>
 __device__ __forceinline__ long long paged_scan(const PagedArgs& a, long long* sums, int& lo, int& hi, long long& before) {
   const int share = (a.batch + kThreads - 1) / kThreads;
   lo = min((int)threadIdx.x * share, a.batch);
   hi = min(lo + share, a.batch);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
+  for (int b = lo; b < hi; ++b)
+    mine += paged_tiles(kEarly ? __ldcg(a.seq_lens + b) : __ldg(a.seq_lens + b), a.max_pages);
   long long upto = mine;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
@@ -111,7 +113,7 @@ template <int kThreads>
 __device__ __forceinline__ void paged_find_range(const PagedArgs& a, int range, long long* sums, PagedRange* out) {
   int lo, hi;
   long long before;
-  const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
+  const long long total = paged_scan<kThreads, false>(a, sums, lo, hi, before);
   const long long per = paged_units(a, total), v0 = range * per, v1 = v0 + per;
   if (threadIdx.x == 0) {
     // (a range behind the last unit has no tiles)
@@ -140,13 +142,13 @@ template <int kThreads>
 __device__ __forceinline__ void paged_find_segments(const PagedArgs& a, int b, long long* sums, PagedSegments* out) {
   int lo, hi;
   long long before;
-  const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
+  const long long total = paged_scan<kThreads, true>(a, sums, lo, hi, before);
   if (b < lo || b >= hi) return;
   const long long per = paged_units(a, total);
-  for (int k = lo; k < b; ++k) before += paged_tiles(__ldg(a.seq_lens + k), a.max_pages);
+  for (int k = lo; k < b; ++k) before += paged_tiles(__ldcg(a.seq_lens + k), a.max_pages);
   const long long first = paged_first_unit(a, b, before);
   out->first = (int)paged_div(first, per);
-  out->count = (int)paged_div(first + paged_tiles(__ldg(a.seq_lens + b), a.max_pages) - 1, per) - out->first + 1;
+  out->count = (int)paged_div(first + paged_tiles(__ldcg(a.seq_lens + b), a.max_pages) - 1, per) - out->first + 1;
 }
 
 }  // namespace dsa

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kWeighThreads)
 paged_weights_kernel(const PagedArgs a, const float* weights, int64_t stride, float* out, int64_t out_stride) {
   __shared__ float lse_sh[kWeighThreads];
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int len = paged_len(__ldg(a.seq_lens + b), a.max_pages);      // older than the attention, as above
+  const int len = paged_len(__ldcg(a.seq_lens + b), a.max_pages);     // older than the attention, as above
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   if ((int64_t)blockIdx.x * kWeighTokens >= len) return;

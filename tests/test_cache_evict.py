@@ -139,6 +139,14 @@ def test_ties_zeros_and_odd_values():
 
 
 @pytest.mark.gpu
+def test_length_beyond_the_table_and_below_zero():
+    args = list(make([300, 200], 100, seed=11))
+    args[1] = torch.tensor([100000, -3], dtype=torch.int32, device="cuda")
+    lens, _, kept = check(args, 100, 3, 10, "cut")
+    assert lens.tolist() == [100, 0] and kept[0, -1] == 319       # the table's last position
+
+
+@pytest.mark.gpu
 def test_requests_within_the_budget_may_keep_their_pages():
     args = list(make([100, 900, 64], 300, seed=5))
     for b in (0, 2):
