@@ -422,9 +422,23 @@ static bool paged_shape_ok(int batch, int tokens, int heads, int max_pages) {
   return batch >= 0 && batch <= 65535 && tokens >= 1 && heads >= 1 && heads <= 128 && (int64_t)tokens * heads <= 65536 &&
          max_pages >= 1 && max_pages <= DSA_PAGED_MAX_PAGES;
 }
+// Whether requests stay whole, from the batch and the width of the block table (the lengths are on the device).  With f
+// CTAs' worth of requests per SM and p pages each, a CTA that takes whole requests is done after ceil(f) of them, about
+// 1.6 p + 3.5 us each; cut ones take f (1.6 p + 5) us, and 10 us for partial results and their join.  The second
+// condition bounds what is lost where most requests are much shorter than the table.  Measured, cut / whole, 16 rows:
+// 1 x 2 pages 11.0 / 9.0 us, 1 x 6 12.3 / 15.8, 64 x 8 22.6 / 20.5, 64 x 16 28.8 / 32.8, 148 x 8 34.2 / 22.6, 160 x 16 53 / 62,
+// 300 x 4 51 / 35, 700 x 8 135 / 86; lengths of 1 to p pages: 160 x 16 32 / 39, 300 x 16 50 / 43, 700 x 24 105 / 84.
+static int paged_split(int batch, int blocks, int max_pages) {
+  const int sms = dsa::sm_count();
+  const int64_t ctas = (int64_t)batch * blocks;
+  const double f = (double)ctas / sms, turns = (double)((ctas + sms - 1) / sms);
+  if (max_pages > 8 + 5 * f || 1.6 * max_pages * (turns - f) > 5 * f - 3.5 * turns + 10) return dsa::kPagedCut;
+  return ctas <= sms ? dsa::kPagedOne : dsa::kPagedSnap;
+}
 // Ranges that the tiles are cut into: a CTA per SM over all row blocks, so that the blocks of one request walk its
 // pages at the same time and share them through L2.
 static int paged_ranges(int batch, int blocks, int max_pages) {
+  if (paged_split(batch, blocks, max_pages) == dsa::kPagedOne) return batch;
   int x = dsa::sm_count() / blocks;
   const int64_t tiles = (int64_t)batch * max_pages;
   if (x > tiles) x = (int)tiles;
@@ -432,9 +446,11 @@ static int paged_ranges(int batch, int blocks, int max_pages) {
   return x < 1 ? 1 : x;
 }
 static int paged_blocks(int rows) { return (rows + dsa::paged_block_rows(rows) - 1) / dsa::paged_block_rows(rows); }
+// [ segments of the requests | partial results | logits ]
+static size_t paged_segment_bytes(int batch) { return round256((size_t)batch * sizeof(int2)); }
 static size_t paged_part_bytes(int batch, int rows, int max_pages) {
   const int blocks = paged_blocks(rows);
-  return round256((size_t)paged_ranges(batch, blocks, max_pages) * blocks * 2 * dsa::paged_part_floats(dsa::paged_block_rows(rows)) * 4);
+  return paged_segment_bytes(batch) + round256((size_t)paged_ranges(batch, blocks, max_pages) * blocks * 2 * dsa::paged_part_floats(dsa::paged_block_rows(rows)) * 4);
 }
 
 size_t dsa_paged_attn_workspace_bytes(int batch, int tokens_per_request, int heads, int max_pages, int with_weights) {
@@ -474,7 +490,8 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
   a.table_stride = block_table_stride;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
-  a.part = static_cast<float*>(workspace);
+  a.segments = static_cast<int2*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_segment_bytes(batch));
   a.logits = new_token_weights ? reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_part_bytes(batch, rows, max_pages))
                                : nullptr;
   a.status = status_dev;
@@ -487,10 +504,11 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
   a.tokens = tokens_per_request;
   a.block_rows = dsa::paged_block_rows(rows);
   a.grid_x = paged_ranges(batch, paged_blocks(rows), max_pages);
+  a.whole = paged_split(batch, paged_blocks(rows), max_pages);
   a.switch_cost = dsa::paged_switch_cost(rows);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = a.block_rows == 64 ? dsa::launch_paged_attn_tc(a, ckv, kpe, s) : dsa::launch_paged_attn_mma(a, ckv, kpe, s);
-  if (e == cudaSuccess && a.grid_x > 1) e = dsa::launch_paged_join(a, s);
+  if (e == cudaSuccess && a.grid_x > 1 && a.whole == dsa::kPagedCut) e = dsa::launch_paged_join(a, s);
   if (e == cudaSuccess && new_token_weights)
     e = dsa::launch_paged_weights(a, token_weights, token_weights_stride, new_token_weights, new_token_weights_stride, s);
   return static_cast<int>(e);

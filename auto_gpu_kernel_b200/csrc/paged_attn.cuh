@@ -21,6 +21,7 @@ struct PagedArgs {
   int64_t table_stride;
   __nv_bfloat16* out;
   float* lse;
+  int2* segments;   // [batch] first range and number of the ranges that a request is cut into
   float* part;      // partial results of cut requests
   float* logits;    // base-2 logits [batch][max_pages][row blocks][rows of a block][64], or null
   int32_t* status;
@@ -30,10 +31,18 @@ struct PagedArgs {
   int heads, tokens;
   int block_rows;   // query rows that a CTA takes at once (a row block)
   int grid_x;       // ranges the tiles are cut into
+  int whole;        // PagedSplit: whether and how requests stay whole
   int switch_cost;  // what taking up a request costs, in tiles
 };
 
 constexpr int kPagedMaxRanges = 512;
+
+// Short requests are better left whole: nothing is written for a join, and the join's launch goes.
+enum PagedSplit {
+  kPagedCut = 0,    // ranges cut requests
+  kPagedOne = 1,    // range r is request r
+  kPagedSnap = 2,   // a range takes the requests that begin in it
+};
 
 // Query rows that a CTA takes at once, from the rows of a request: 16 by warp-level products, 64 by tcgen05.  At 16 rows the
 // first keeps three pages in shared memory where the second has room for two beside its q (64 x 32768 tokens 363 us
@@ -54,24 +63,22 @@ __host__ __device__ inline int paged_tiles(int len, int max_pages) {
 }
 
 // Partial results: per (row block, range, which) a [rows of the block][512] fp32 accumulator ([16][512][4] for blocks of
-// 64 rows: four rows, column, row of the four), then its running maxima and sums.  `which` is 1 for the segment a request begins with and 0 for the ones that follow: a range
-// holds at most one of each.
+// 64 rows: four rows, column, row of the four), then its running maxima and sums.  `which` is 1 for the segment a
+// request begins with and 0 for the ones that follow: a range holds at most one of each.
 __host__ __device__ inline size_t paged_part_floats(int block_rows) { return (size_t)block_rows * (kCkv + 2); }
 __device__ __forceinline__ float* paged_part(const PagedArgs& a, int block_rows, int rb, int range, int which) {
   return a.part + (((size_t)rb * a.grid_x + range) * 2 + which) * paged_part_floats(block_rows);
 }
 
 // Sum of all requests' tiles, and the tiles in front of this thread's share of the requests (requests
-// [lo, hi) of equal contiguous shares).  By all threads of the CTA; `sums` has one entry per warp.  kEarly: in front of the
-// dependency wait, past L1.
-template <int kThreads, bool kEarly>
+// [lo, hi) of equal contiguous shares).  By all threads of the CTA; `sums` has one entry per warp.
+template <int kThreads>
 __device__ __forceinline__ long long paged_scan(const PagedArgs& a, long long* sums, int& lo, int& hi, long long& before) {
   const int share = (a.batch + kThreads - 1) / kThreads;
   lo = min((int)threadIdx.x * share, a.batch);
   hi = min(lo + share, a.batch);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b)
-    mine += paged_tiles(kEarly ? __ldcg(a.seq_lens + b) : __ldg(a.seq_lens + b), a.max_pages);
+  for (int b = lo; b < hi; ++b) mine += paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
   long long upto = mine;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
@@ -107,15 +114,40 @@ __device__ __forceinline__ long long paged_first_unit(const PagedArgs& a, int b,
 // all requests).  By all threads of the CTA; a __syncthreads must follow before the words are read.
 struct PagedRange {
   long long begin, end;
+  long long unit, per;      // the first tile's unit, units of a range
   int start_b, start_j;
 };
 template <int kThreads>
 __device__ __forceinline__ void paged_find_range(const PagedArgs& a, int range, long long* sums, PagedRange* out) {
+  if (a.whole == kPagedOne) {
+    if (threadIdx.x == 0) *out = {0, paged_tiles(__ldg(a.seq_lens + range), a.max_pages), 0, 1, range, 0};
+    return;
+  }
+  if (threadIdx.x == 0) out->begin = out->end = 0;      // a range without a request (the scan holds a barrier)
   int lo, hi;
   long long before;
-  const long long total = paged_scan<kThreads, false>(a, sums, lo, hi, before);
+  const long long total = paged_scan<kThreads>(a, sums, lo, hi, before);
   const long long per = paged_units(a, total), v0 = range * per, v1 = v0 + per;
+  if (a.whole == kPagedSnap) {
+    int ahead = lo > 0 ? paged_tiles(__ldg(a.seq_lens + lo - 1), a.max_pages) : 0;    // tiles of the request before
+    for (int b = lo; b < hi; ++b) {
+      const int k = paged_tiles(__ldg(a.seq_lens + b), a.max_pages);
+      const long long first = paged_first_unit(a, b, before);
+      if (first >= v0 && first < v1) {
+        if (b == 0 || first - a.switch_cost - ahead < v0) {
+          out->begin = before;
+          out->start_b = b;
+          out->start_j = 0;
+        }
+        if (b == a.batch - 1 || first + k + a.switch_cost >= v1) out->end = before + k;
+      }
+      before += k;
+      ahead = k;
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
+    out->per = per;
     // (a range behind the last unit has no tiles)
     if (v0 >= total + (long long)a.batch * a.switch_cost) out->begin = total;
     if (v1 >= total + (long long)a.batch * a.switch_cost) out->end = total;
@@ -126,6 +158,7 @@ __device__ __forceinline__ void paged_find_range(const PagedArgs& a, int range, 
     if (v0 >= begin && v0 < end) {
       const int j = v0 > first ? (int)(v0 - first) : 0;
       out->begin = before + j;
+      out->unit = first + j;
       out->start_b = b;
       out->start_j = j;
     }
@@ -134,21 +167,10 @@ __device__ __forceinline__ void paged_find_range(const PagedArgs& a, int range, 
   }
 }
 
-// The segments of request b: ranges first .. first + count - 1.  By all threads of the CTA, the same contract.
-struct PagedSegments {
-  int first, count;
-};
-template <int kThreads>
-__device__ __forceinline__ void paged_find_segments(const PagedArgs& a, int b, long long* sums, PagedSegments* out) {
-  int lo, hi;
-  long long before;
-  const long long total = paged_scan<kThreads, true>(a, sums, lo, hi, before);
-  if (b < lo || b >= hi) return;
-  const long long per = paged_units(a, total);
-  for (int k = lo; k < b; ++k) before += paged_tiles(__ldcg(a.seq_lens + k), a.max_pages);
-  const long long first = paged_first_unit(a, b, before);
-  out->first = (int)paged_div(first, per);
-  out->count = (int)paged_div(first + paged_tiles(__ldcg(a.seq_lens + b), a.max_pages) - 1, per) - out->first + 1;
+// By the CTA of the first row block that has a request's first tile, its tile `i`: what the join needs to know of it.
+__device__ __forceinline__ void paged_tell_segments(const PagedArgs& a, const PagedRange& r, int range, int i, int b, int len) {
+  const long long first = r.unit + i + (long long)(b - r.start_b) * a.switch_cost;
+  a.segments[b] = make_int2(range, (int)paged_div(first + paged_tiles(len, a.max_pages) - 1, r.per) - range + 1);
 }
 
 }  // namespace dsa

@@ -199,6 +199,8 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
       l0 = l1 = 0.f;
       cur_b = tile.b;
       first_j = tile.j;
+      if (tid == 0 && rb == 0 && first_j == 0 && a.whole == kPagedCut)
+        paged_tell_segments(a, sh.range, range, i, tile.b, tile.len);
       const int base = tile.len - a.tokens + 1;
       lim0 = row_tok[0] < 0 ? 0 : base + row_tok[0];
       lim1 = row_tok[1] < 0 ? 0 : base + row_tok[1];

@@ -147,6 +147,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
       if (tile.b != cur_b) {
         cur_b = tile.b;
         first_j = tile.j;
+        if (tid == 0 && rb == 0 && first_j == 0 && a.whole == kPagedCut)
+          paged_tell_segments(a, sh.range, range, i, tile.b, tile.len);
         seg_live = 0;
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.f;

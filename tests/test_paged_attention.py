@@ -126,6 +126,18 @@ def test_many_requests_share_a_cta():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,most,heads,extra", [(148, 300, 16, 0), (149, 300, 16, 0), (297, 130, 16, 0), (300, 200, 16, 60),
+                                                    (500, 64, 5, 0), (1100, 70, 16, 40), (30, 500, 64, 0), (200, 130, 48, 0),
+                                                    (160, 150, 33, 50), (75, 200, 100, 0)])
+def test_requests_left_whole_and_cut(batch, most, heads, extra):
+    """One request per CTA, several per CTA, and (in a table much wider than the lengths) ranges that cut them."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, most + 1, (batch,), generator=gen).tolist()
+    lens[0], lens[-1] = most, 0
+    run_and_check(make(lens, heads=heads, seed=batch, extra_cols=extra), f"{batch} x {most}, {heads} heads", weights=batch % 2 == 0)
+
+
+@pytest.mark.gpu
 def test_one_long_request_over_all_ctas():
     run_and_check(make([70001], seed=3), "70001 tokens", weights=True)
 
