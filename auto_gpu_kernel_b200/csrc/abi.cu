@@ -449,8 +449,10 @@ static int paged_blocks(int rows) { return (rows + dsa::paged_block_rows(rows) -
 // [ segments of the requests | partial results | logits ]
 static size_t paged_segment_bytes(int batch) { return round256((size_t)batch * sizeof(int2)); }
 static size_t paged_part_bytes(int batch, int rows, int max_pages) {
-  const int blocks = paged_blocks(rows);
-  return paged_segment_bytes(batch) + round256((size_t)paged_ranges(batch, blocks, max_pages) * blocks * 2 * dsa::paged_part_floats(dsa::paged_block_rows(rows)) * 4);
+  const int blocks = paged_blocks(rows), ranges = paged_ranges(batch, blocks, max_pages);
+  if (ranges == 1 || paged_split(batch, blocks, max_pages) != dsa::kPagedCut) return paged_segment_bytes(batch);
+  return paged_segment_bytes(batch) +
+         round256((size_t)ranges * blocks * 2 * dsa::paged_part_floats(dsa::paged_block_rows(rows)) * sizeof(float));
 }
 
 size_t dsa_paged_attn_workspace_bytes(int batch, int tokens_per_request, int heads, int max_pages, int with_weights) {

@@ -88,7 +88,9 @@ def test_workspace_holds_partials_and_logits():
     plain, logits = size(64, 1, 16, 512, 0), size(64, 1, 16, 512, 1)
     assert logits - plain == 64 * 512 * 16 * 64 * 4        # fp32 logits of every cached token and query row
     assert plain % 256 == 0
-    assert size(1, 1, 16, 1, 0) >= 2 * 16 * 514 * 4
+    assert size(1, 1, 16, 64, 0) >= 64 * 2 * 16 * 514 * 4   # a request over 64 CTAs
+    assert size(1, 1, 16, 1, 0) == 256                     # whole requests leave no partial results
+    assert size(1, 4096, 16, 512, 0) == 256                # nor do more row blocks than SMs
 
 
 def test_cpu_tensors_are_refused():
@@ -116,6 +118,12 @@ def test_head_counts(heads):
 def test_several_new_tokens(tokens, heads):
     # requests shorter than their new tokens: the first of these see nothing
     run_and_check(make([257, 64, 1, 2, 0, 66, 700], heads=heads, tokens=tokens, seed=tokens), f"{tokens} tokens", weights=True)
+
+
+@pytest.mark.gpu
+def test_a_prompt_chunk():
+    """More row blocks than SMs: every CTA walks the whole cache."""
+    run_and_check(make([1500, 700], tokens=640, seed=40), "640 tokens", weights=True)
 
 
 @pytest.mark.gpu
