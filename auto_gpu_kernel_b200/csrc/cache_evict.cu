@@ -198,13 +198,15 @@ evict_choose_kernel(const EvictArgs a) {
   if (csize > 1) cluster.sync();         // nobody leaves while its counts may be read
 }
 
-// CTAs per request: up to four while the SMs hold them at once and a slice stays 4096 keys; less is not worth the
-// cluster's barriers.  Whole call with 512 or 1024 kept tokens, 1 / 2 / 4 CTAs: 1 x 4096 tokens 12.3 / 14.3 / 14.4 us,
-// 4 x 8192 16.4 / 14.9 / 16.4, 64 x 16384 36.4 / 32.3 / 34.9, 128 x 8192 42.1 / 44.4 / 60.1, 16 x 32768 32.8 / 24.6 / 21.1,
-// 32 x 32768 39.9 / 30.7 / 26.7 (eight were slower throughout).
+// CTAs per request: up to four while the SMs hold them at once and a slice stays 4096 keys, eight while it stays 16384 (a
+// cluster of eight needs its SMs inside one GPC, and fewer fit); less is not worth the cluster's barriers.  Whole call with
+// 512 or 1024 kept tokens, 1 / 2 / 4 CTAs: 1 x 4096 tokens 12.3 / 14.3 / 14.4 us, 4 x 8192 16.4 / 14.9 / 16.4, 64 x 16384
+// 36.4 / 32.3 / 34.9, 128 x 8192 42.1 / 44.4 / 60.1, 16 x 32768 32.8 / 24.6 / 21.1, 32 x 32768 39.9 / 30.7 / 26.7; 4 / 8 CTAs:
+// 8 x 65536 26.7 / 26.6, 14 x 131072 43.1 / 36.9, 1 x 1000000 307 / 169.
 int ev_cluster(int batch, int64_t longest, int sms) {
   int c = 1;
-  while (c < 4 && longest / (2 * c) >= 4096 && (int64_t)batch * 2 * c <= sms * 9 / 10) c *= 2;
+  while (c < 8 && longest / (2 * c) >= (c < 4 ? 4096 : 16384) && (int64_t)batch * 2 * c <= (c < 4 ? sms * 9 / 10 : sms * 8 / 10))
+    c *= 2;
   return c;
 }
 

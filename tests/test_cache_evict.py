@@ -109,9 +109,16 @@ def test_budgets(budget, first, last):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("lens,budget", [([5000, 4097, 8200], 4096), ([70001], 9000), ([20000, 3, 16384], 2048)])
+@pytest.mark.parametrize("lens,budget", [([5000, 4097, 8200], 4096), ([70001], 9000), ([20000, 3, 16384], 2048),
+                                         ([140000, 131000], 3000), ([400003], 50), ([9000] * 20, 64),
+                                         ([400003], 150), ([9000] * 20, 164)])
 def test_long_rows(lens, budget):
-    check(make(lens, budget, seed=len(lens), index=len(lens) != 3), budget, 4, 100, str(lens))
+    args = make(lens, budget, seed=len(lens), index=len(lens) != 3)
+    if budget < 104:                                     # what is always kept does not fit: refused
+        with pytest.raises(ValueError, match="keep_first"):
+            check(args, budget, 4, 100, str(lens))
+        return
+    check(args, budget, 4, 100, str(lens))
 
 
 @pytest.mark.gpu
