@@ -12,6 +12,8 @@ import torch
 from . import _lib, workspace
 from .paged_attention import PAGE, caches_ok, refuse_caches, refuse_tables, rows_of, tables_ok
 
+MAX_BUDGET = 1 << 30
+
 
 def _evict(token_weights, seq_lens, block_table, new_block_table, budget, ckv_cache, kpe_cache, k_index_cache_fp8,
            new_seq_lens, new_token_weights, kept_positions, keep_first, keep_last):
@@ -20,8 +22,8 @@ def _evict(token_weights, seq_lens, block_table, new_block_table, budget, ckv_ca
         raise RuntimeError(f"{what}: CUDA tensors required (this operator has no CPU path)")
     index = token_weights.get_device()
     budget = int(budget)
-    if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
-        raise ValueError(f"{what}: budget >= 1 and 0 <= keep_first + keep_last <= budget")
+    if not 1 <= budget <= MAX_BUDGET or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+        raise ValueError(f"{what}: 1 <= budget <= 2^30 and 0 <= keep_first + keep_last <= budget")
     if not tables_ok(seq_lens, block_table, index):
         refuse_tables(what, seq_lens, block_table, index)
     if not tables_ok(seq_lens, new_block_table, index):

@@ -442,7 +442,6 @@ static int paged_ranges(int batch, int blocks, int max_pages) {
   int x = dsa::sm_count() / blocks;
   const int64_t tiles = (int64_t)batch * max_pages;
   if (x > tiles) x = (int)tiles;
-  if (x > dsa::kPagedMaxRanges) x = dsa::kPagedMaxRanges;
   return x < 1 ? 1 : x;
 }
 static int paged_blocks(int rows) { return (rows + dsa::paged_block_rows(rows) - 1) / dsa::paged_block_rows(rows); }
@@ -528,7 +527,7 @@ int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, co
     return DSA_ERR_NULL_POINTER;
   const int64_t width = (int64_t)max_pages * dsa::kPage, most = width < budget ? width : budget;
   if (batch < 0 || batch > 65535 || max_pages < 1 || max_pages > DSA_PAGED_MAX_PAGES || num_pages <= 0 ||
-      num_pages > DSA_PAGED_MAX_PAGES || budget < 1 || keep_first < 0 || keep_last < 0 ||
+      num_pages > DSA_PAGED_MAX_PAGES || budget < 1 || budget > DSA_EVICT_MAX_BUDGET || keep_first < 0 || keep_last < 0 ||
       (int64_t)keep_first + keep_last > budget || (int64_t)new_max_pages * dsa::kPage < most || token_weights_stride < width ||
       new_token_weights_stride < budget || kept_stride < budget || block_table_stride < 0 || new_block_table_stride < 0)
     return DSA_ERR_BAD_SHAPE;

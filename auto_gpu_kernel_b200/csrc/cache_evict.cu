@@ -229,8 +229,10 @@ evict_move_kernel(const EvictArgs a) {
   if (lane < kMvRows && j0 + lane < m) {
     const int j = j0 + lane;
     const int from = __ldcg(a.kept + (int64_t)b * a.kept_stride + j);
-    a.new_weights[(int64_t)b * a.new_weights_stride + j] = __ldg(a.weights + (int64_t)b * a.weights_stride + from);
-    const int p = __ldg(a.table + (int64_t)b * a.table_stride + from / kPage);
+    // (a caller whose outputs overlap has written over the choice: nothing out of bounds is read for it)
+    const bool known = from >= 0 && from < n;
+    if (known) a.new_weights[(int64_t)b * a.new_weights_stride + j] = __ldg(a.weights + (int64_t)b * a.weights_stride + from);
+    const int p = known ? __ldg(a.table + (int64_t)b * a.table_stride + from / kPage) : -1;
     const int q = __ldg(a.new_table + (int64_t)b * a.new_table_stride + j / kPage);
     if (p < 0 || p >= a.num_pages || q < 0 || q >= a.num_pages) {
       raise_status(a.status, DSA_STATUS_BAD_PAGE);

@@ -35,8 +35,6 @@ struct PagedArgs {
   int switch_cost;  // what taking up a request costs, in tiles
 };
 
-constexpr int kPagedMaxRanges = 512;
-
 // Short requests are better left whole: nothing is written for a join, and the join's launch goes.
 enum PagedSplit {
   kPagedCut = 0,    // ranges cut requests

@@ -156,7 +156,7 @@ paged_join_kernel(const PagedArgs a) {
 
 // Four cached tokens per thread, 1024 of one request per CTA; a row's 64 logits of a page are one coalesced 256-byte
 // read, and the rows are added in ascending order.  64 x 16384 tokens, 16 rows (67 MB of logits just written, so most of them
-// from L2, 4 MB of weights in and out): 14 us.
+// from L2, 4 MB of weights in and out): 16 us.
 constexpr int kWeighThreads = 256;
 constexpr int kWeighTokens = 4 * kWeighThreads;
 __global__ void __launch_bounds__(kWeighThreads)

@@ -238,7 +238,10 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
  * from, unless every kept token on it keeps its place (a request within the budget may pass its old row and
  * nothing moves), nor stand twice in new_block_table: such moves race.  The outputs must not overlap the inputs.
  * Page ids outside [0, num_pages) are skipped (DSA_STATUS_BAD_PAGE).
+ * max_pages, num_pages <= DSA_PAGED_MAX_PAGES; budget <= DSA_EVICT_MAX_BUDGET (the tokens of as many pages).
  * ------------------------------------------------------------------------------------------- */
+#define DSA_EVICT_MAX_BUDGET (1 << 30)
+
 int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, const int32_t* seq_lens,
                     const int32_t* block_table, int64_t block_table_stride, const int32_t* new_block_table,
                     int64_t new_block_table_stride, void* ckv, void* kpe, void* k_index_cache,

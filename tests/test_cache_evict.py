@@ -79,7 +79,8 @@ def test_host_side_argument_errors():
         assert call(**{name: None}) == -1, name
     for kw in (dict(ws=511), dict(ts=-1), dict(ns=-1), dict(nws=199), dict(ks=199), dict(b=-1), dict(b=65536), dict(mp=0),
                dict(mp=(1 << 24) + 1), dict(nmp=3), dict(pages=0), dict(budget=0), dict(first=-1), dict(last=-1),
-               dict(first=137, last=64), dict(pages=(1 << 24) + 1)):
+               dict(first=137, last=64), dict(pages=(1 << 24) + 1),
+               dict(budget=(1 << 30) + 1, nws=1 << 31, ks=1 << 31, nmp=1 << 25)):
         assert call(**kw) == -2, kw
     for name in ("c", "k", "i"):
         assert call(**{name: 8}) == -4, name
@@ -235,6 +236,8 @@ def test_refusals():
             cache_evict.run(*a, **kw)
     refuses(ValueError, w, lens, table, new, 0, ckv, kpe, keys)
     refuses(ValueError, w, lens, table, new, 100, ckv, kpe, keys, 60, 50)
+    refuses(ValueError, w, lens, table, new, 2 ** 30 + 1, ckv, kpe, keys)
+    refuses(ValueError, w, lens, table, new, 2 ** 32 + 100, ckv, kpe, keys)
     refuses(ValueError, w, lens, table, new, 100, ckv, kpe, keys, -1, 0)
     refuses(ValueError, w, lens, table, new, 200, ckv, kpe, keys)                 # two new pages hold 128 tokens
     refuses(ValueError, w[:, :300], lens, table, new, 100, ckv, kpe, keys)
