@@ -125,6 +125,8 @@ def _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale,
     rows, heads, _ = shape
     batch, max_pages = block_table.shape
     if rows == 0:
+        if batch and new_token_weights is not None:
+            raise ValueError(f"paged attention: no query tokens whose weights {batch} requests could receive")
         return output, lse
     if batch == 0 or rows % batch:
         raise ValueError(f"paged attention: {rows} query tokens are no multiple of the {batch} requests")
@@ -164,7 +166,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     q_nope [B*n,heads,512] / q_pe [B*n,heads,64] bf16: the n newest tokens of every request, oldest first (1 to 128
     heads).  `seq_lens` counts the cached tokens of each request, the new ones among them: token i of n sees the
     positions below seq_len - n + 1 + i, and one that sees none gets output 0 and lse -inf.  Cache rows at or
-    behind seq_len may hold anything, those in front of it must be finite.
+    behind seq_len may hold anything, those in front of it must be finite.  The outputs must not overlap the inputs
+    or one another.
 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of

@@ -388,5 +388,6 @@ def test_refusals():
     refuses(ValueError, a0=flat[:args[0].numel()].view(args[0].shape), output=flat[512:].view(args[0].shape))
     empty = paged_attention.run(args[0][:0], args[1][:0], *args[2:4], args[4][:0], args[5][:0], SCALE)
     assert empty[0].shape == (0, 16, 512)
+    refuses(ValueError, a0=args[0][:0], a1=args[1][:0], new_token_weights=w)          # two requests, no query token
     none = paged_attention.run(*args[:5], args[5][:, :0], SCALE)
     assert (none[0] == 0).all() and torch.isinf(none[1]).all()
