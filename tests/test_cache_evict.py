@@ -227,6 +227,68 @@ def test_streams_and_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,budget", [([3000, 40, 5000], 700), ([90000, 20000], 9000)])
+def test_moved_rows_on_another_stream_and_in_a_replay(lens, budget):
+    """The rows themselves, from pages that held something else before each run."""
+    from auto_gpu_kernel_b200 import cache_evict, workspace
+    weights, seq_lens, table, _, ckv, kpe, keys = make([max(lens)] * len(lens), budget, seed=12)
+    seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    per = -(-budget // PAGE)
+    used = torch.zeros(ckv.shape[0], dtype=torch.bool)
+    used[table.cpu().long().flatten()] = True
+    new = (~used).nonzero().flatten()[:per * len(lens)].view(len(lens), per).to(torch.int32).cuda()
+    caches = (ckv.view(-1, 512), kpe.view(-1, 64), keys.view(-1, PAGE * 132))
+
+    def forget():
+        caches[0].view(-1, PAGE, 512)[new.long()] = -1.25
+        caches[1].view(-1, PAGE, 64)[new.long()] = 3.5
+        caches[2][new.long()] = 77
+
+    def expect(lens):
+        """What the caches hold after a move, from the plain choice and the old pages."""
+        want = [c.clone() for c in caches]
+        for b, n in enumerate(lens):
+            mine = torch.tensor(po.evict_choice(weights[b], n, budget, 4, 64), device="cuda")
+            src, dst = po.slots_of(table[b], n)[mine], po.slots_of(new[b], len(mine))
+            want[0][dst], want[1][dst] = caches[0][src], caches[1][src]
+            for width, at in ((128, 0), (4, PAGE * 128)):
+                byte = torch.arange(width, device="cuda")
+                want[2][(dst // PAGE)[:, None], at + (dst % PAGE)[:, None] * width + byte] = \
+                    caches[2][(src // PAGE)[:, None], at + (src % PAGE)[:, None] * width + byte]
+        return want
+
+    def same(want, label):
+        for name, got, w in zip(("ckv", "kpe", "index keys"), caches, want):
+            assert torch.equal(bits(got), bits(w)), f"{label}: {name}"
+
+    def call():
+        return cache_evict.run(weights, seq_lens, table, new, budget, ckv, kpe, keys, 4, 64)
+    call()
+    torch.cuda.synchronize()
+    forget()
+    want = expect(lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    same(want, "another stream")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = call()
+    for shorter in (lens, [n - 17 for n in lens], lens[::-1]):
+        forget()
+        weights.copy_(torch.rand_like(weights))
+        seq_lens.copy_(torch.tensor(shorter, dtype=torch.int32))
+        want = expect(shorter)
+        g.replay()
+        torch.cuda.synchronize()
+        same(want, f"replay with {shorter}")
+        assert res[0].tolist() == [min(n, budget) for n in shorter]
+    assert workspace.check_status() == 0
+
+
+@pytest.mark.gpu
 def test_refusals():
     from auto_gpu_kernel_b200 import cache_evict
     w, lens, table, new, ckv, kpe, keys = make([400, 300], 100, seed=10)
