@@ -18,6 +18,8 @@ _c_size = ctypes.c_size_t
 _ptr = ctypes.c_void_p
 _c_float = ctypes.c_float
 
+ERR_OVERLAP = -7
+
 # name -> (restype, argtypes); mirrors include/dsa_b200.h one to one.
 SIGNATURES = {
     "dsa_b200_version": (_c_int, []),
@@ -131,7 +133,7 @@ def load(build_if_missing: bool = True):
 
 
 def check(code: int, what: str):
-    """Turn a non-zero return code of the C ABI into a RuntimeError."""
+    """Turn a non-zero return code of the C ABI into a RuntimeError (a ValueError where arguments overlap)."""
     if code != 0:
         text = load().dsa_b200_error_string(code).decode()
-        raise RuntimeError(f"{what}: {text} (code {code})")
+        raise (ValueError if code == ERR_OVERLAP else RuntimeError)(f"{what}: {text} (code {code})")

@@ -49,15 +49,11 @@ def _evict(token_weights, seq_lens, block_table, new_block_table, budget, ckv_ca
     elif new_seq_lens.dim() != 1 or new_seq_lens.shape[0] != batch or new_seq_lens.dtype is not torch.int32 \
             or not new_seq_lens.is_contiguous() or new_seq_lens.get_device() != index:
         raise ValueError(f"{what}: new_seq_lens must be a contiguous [B] int32 tensor on cuda:{index}")
-    elif workspace.overlap(seq_lens, new_seq_lens):
-        raise ValueError(f"{what}: the outputs must not overlap the inputs")
     if new_token_weights is None:
         new_token_weights = token_weights.new_empty((batch, budget))
         nw, nw_stride = new_token_weights.data_ptr(), budget
     else:
         nw, nw_stride = rows_of(what, "new_token_weights", new_token_weights, batch, budget, torch.float32, index)
-        if workspace.overlap(token_weights, new_token_weights):
-            raise ValueError(f"{what}: the outputs must not overlap the inputs")
     if kept_positions is None:
         kept_positions = seq_lens.new_empty((batch, budget))
         kept, kept_stride = kept_positions.data_ptr(), budget
@@ -94,7 +90,8 @@ def kernel(token_weights, seq_lens, block_table, new_block_table, budget, ckv_ca
 
     A page of new_block_table must not be one that a request of this call still reads from, unless every kept
     token on it keeps its place (a request within the budget may pass its old row: nothing moves then), and must
-    not stand in it twice: such moves race."""
+    not stand in it twice: such moves race.  Outputs that share memory with an input, a cache or one another are
+    refused."""
     if new_seq_lens is None or new_token_weights is None or kept_positions is None:
         raise ValueError("cache eviction: kernel() needs its three outputs")
     _evict(token_weights, seq_lens, block_table, new_block_table, budget, ckv_cache, kpe_cache, k_index_cache_fp8, new_seq_lens,

@@ -58,6 +58,32 @@ cudaError_t launch_rotary_append(const void*, int64_t, int64_t, const void*, int
 namespace {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Memory of an argument: `rows` rows of `row` bytes, `stride` bytes apart.
+struct Region {
+  const void* at;
+  size_t row, stride, rows;
+};
+// Whether two arguments may share a byte.  Exact for rows of one pitch (column ranges of one buffer are apart although their
+// spans meet); for others it goes by the spans.
+inline bool meet(const Region& a, const Region& b) {
+  if (a.at == nullptr || b.at == nullptr || a.row == 0 || b.row == 0 || a.rows == 0 || b.rows == 0) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.at), pb = reinterpret_cast<uintptr_t>(b.at);
+  if (pa + (a.rows - 1) * a.stride + a.row <= pb || pb + (b.rows - 1) * b.stride + b.row <= pa) return false;
+  const size_t pitch = a.rows > 1 ? a.stride : b.stride;
+  if (pitch == 0 || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return true;
+  const Region &lo = pa <= pb ? a : b, &hi = pa <= pb ? b : a;
+  const size_t off = (pa <= pb ? pb - pa : pa - pb) % pitch;
+  return off < lo.row || off + hi.row > pitch;
+}
+// Whether one of the first `outputs` regions meets any other one.
+template <int kN>
+inline bool outputs_meet(const Region (&r)[kN], int outputs) {
+  for (int i = 0; i < outputs; ++i)
+    for (int j = i + 1; j < kN; ++j)
+      if (meet(r[i], r[j])) return true;
+  return false;
+}
 // score rows are padded to a multiple of 128 tokens so a 2-page tile never crosses rows
 inline int64_t score_row_stride(int max_pages) { return ((int64_t)max_pages * dsa::kPage + 127) / 128 * 128; }
 }  // namespace
@@ -76,6 +102,7 @@ const char* dsa_b200_error_string(int code) {
     case DSA_ERR_UNSUPPORTED: return "dsa_b200: variant not available";
     case DSA_ERR_SCRATCH_TOO_SMALL:
       return "dsa_b200: batch x context exceeds the built-in scratch of dsa_indexer_topk_noalloc";
+    case DSA_ERR_OVERLAP: return "dsa_b200: outputs must not overlap the inputs or one another";
     default: break;
   }
   if (code > 0) return cudaGetErrorString(static_cast<cudaError_t>(code));
@@ -483,6 +510,22 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
   if (workspace_bytes < dsa_paged_attn_workspace_bytes(batch, tokens_per_request, heads, max_pages, new_token_weights != nullptr))
     return DSA_ERR_WORKSPACE_TOO_SMALL;
   const int rows = tokens_per_request * heads;
+  const size_t all_rows = (size_t)batch * rows, slots = (size_t)num_pages * dsa::kPage, held = (size_t)width * sizeof(float);
+  // weights that grow in place are one argument
+  const bool in_place = token_weights == new_token_weights && (batch == 1 || token_weights_stride == new_token_weights_stride);
+  const Region regions[] = {
+      {out, all_rows * dsa::kCkv * 2, 0, 1},
+      {lse, all_rows * sizeof(float), 0, 1},
+      {new_token_weights, held, (size_t)new_token_weights_stride * sizeof(float), (size_t)batch},
+      {workspace, workspace_bytes, 0, 1},
+      {in_place ? nullptr : token_weights, held, (size_t)token_weights_stride * sizeof(float), (size_t)batch},
+      {q_nope, all_rows * dsa::kCkv * 2, 0, 1},
+      {q_pe, all_rows * dsa::kKpe * 2, 0, 1},
+      {ckv, slots * dsa::kCkv * 2, 0, 1},
+      {kpe, slots * dsa::kKpe * 2, 0, 1},
+      {seq_lens, (size_t)batch * sizeof(int32_t), 0, 1},
+      {block_table, (size_t)max_pages * sizeof(int32_t), (size_t)block_table_stride * sizeof(int32_t), (size_t)batch}};
+  if (outputs_meet(regions, 4)) return DSA_ERR_OVERLAP;
   dsa::PagedArgs a = {};
   a.q_nope = static_cast<const __nv_bfloat16*>(q_nope);
   a.q_pe = static_cast<const __nv_bfloat16*>(q_pe);
@@ -532,6 +575,19 @@ int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, co
       new_token_weights_stride < budget || kept_stride < budget || block_table_stride < 0 || new_block_table_stride < 0)
     return DSA_ERR_BAD_SHAPE;
   if (!aligned16(ckv) || !aligned16(kpe) || !aligned16(k_index_cache)) return DSA_ERR_MISALIGNED;
+  const size_t slots = (size_t)num_pages * dsa::kPage, kept_row = (size_t)budget * sizeof(int32_t), n = (size_t)batch;
+  const Region regions[] = {
+      {ckv, slots * dsa::kCkv * 2, 0, 1},
+      {kpe, slots * dsa::kKpe * 2, 0, 1},
+      {k_index_cache, (size_t)num_pages * dsa::kPageBytes, 0, 1},
+      {new_seq_lens, n * sizeof(int32_t), 0, 1},
+      {new_token_weights, kept_row, (size_t)new_token_weights_stride * sizeof(float), n},
+      {kept, kept_row, (size_t)kept_stride * sizeof(int32_t), n},
+      {token_weights, (size_t)width * sizeof(float), (size_t)token_weights_stride * sizeof(float), n},
+      {seq_lens, n * sizeof(int32_t), 0, 1},
+      {block_table, (size_t)max_pages * sizeof(int32_t), (size_t)block_table_stride * sizeof(int32_t), n},
+      {new_block_table, (size_t)new_max_pages * sizeof(int32_t), (size_t)new_block_table_stride * sizeof(int32_t), n}};
+  if (outputs_meet(regions, 6)) return DSA_ERR_OVERLAP;
   return static_cast<int>(dsa::launch_cache_evict(
       token_weights, token_weights_stride, seq_lens, block_table, block_table_stride, new_block_table, new_block_table_stride,
       ckv, kpe, k_index_cache, new_seq_lens, new_token_weights, new_token_weights_stride, kept, kept_stride, batch, max_pages,
@@ -554,6 +610,23 @@ int dsa_rotary_append(const void* q_pe, int64_t q_token_stride, int64_t q_head_s
   if (!aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(q_out) || !aligned16(ckv_cache) ||
       !aligned16(kpe_cache) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0 || ckv_stride % 8 != 0 || kpe_stride % 8 != 0)
     return DSA_ERR_MISALIGNED;
+  const size_t n = (size_t)tokens, q_row = ((size_t)(heads - 1) * q_head_stride + dsa::kKpe) * 2;
+  const bool in_place = q_out == q_pe && (heads == 1 || q_head_stride == dsa::kKpe) &&
+                        (tokens == 1 || q_token_stride == (int64_t)heads * dsa::kKpe);
+  const Region q = {in_place ? nullptr : q_pe, q_row, (size_t)q_token_stride * 2, n};
+  const Region turned = {q_out, n * heads * dsa::kKpe * 2, 0, 1};
+  const Region regions[] = {
+      {ckv_cache, (size_t)num_slots * dsa::kCkv * 2, 0, 1},
+      {kpe_cache, (size_t)num_slots * dsa::kKpe * 2, 0, 1},
+      turned,
+      q,
+      {positions, n * sizeof(int32_t), (size_t)positions_stride * sizeof(int32_t), (size_t)axes},
+      {inv_freq, dsa::kKpe / 2 * sizeof(float), 0, 1},
+      {slots, n * sizeof(int32_t), 0, 1}};
+  // (ckv and kpe may lie in the caches, where rows of another place are stored again)
+  if (outputs_meet(regions, 3) || meet(turned, {ckv, dsa::kCkv * 2, (size_t)ckv_stride * 2, n}) ||
+      meet(turned, {kpe, dsa::kKpe * 2, (size_t)kpe_stride * 2, n}))
+    return DSA_ERR_OVERLAP;
   return static_cast<int>(dsa::launch_rotary_append(q_pe, q_token_stride, q_head_stride, ckv, ckv_stride, kpe, kpe_stride,
                                                     positions, positions_stride, inv_freq, pair_axes, interleaved, slots, q_out,
                                                     ckv_cache, kpe_cache, tokens, heads, num_slots, status_dev,

@@ -116,8 +116,6 @@ def _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale,
         output = q_nope.new_empty((shape[0], shape[1], CKV))
     else:
         _check_output("output", output, shape, bf16, index)
-        if abs(output.data_ptr() - q_nope.data_ptr()) < 2 * q_nope.numel():
-            raise ValueError("paged attention: output must not overlap q_nope")
     if lse is None:
         lse = q_nope.new_empty((shape[0], shape[1]), dtype=torch.float32)
     else:
@@ -139,8 +137,6 @@ def _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale,
             raise ValueError("paged attention: token_weights without new_token_weights")
         old, old_stride = rows_of("paged attention", "token_weights", token_weights, batch, max_pages * PAGE, torch.float32,
                                   index)
-        if (old != new or old_stride != new_stride) and workspace.overlap(token_weights, new_token_weights):
-            raise ValueError("paged attention: token_weights and new_token_weights overlap without being one tensor")
     if max_pages == 0:
         output.zero_()
         lse.fill_(float("-inf"))
@@ -166,8 +162,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     q_nope [B*n,heads,512] / q_pe [B*n,heads,64] bf16: the n newest tokens of every request, oldest first (1 to 128
     heads).  `seq_lens` counts the cached tokens of each request, the new ones among them: token i of n sees the
     positions below seq_len - n + 1 + i, and one that sees none gets output 0 and lse -inf.  Cache rows at or
-    behind seq_len may hold anything, those in front of it must be finite.  The outputs must not overlap the inputs
-    or one another.
+    behind seq_len may hold anything, those in front of it must be finite.  Outputs that share memory
+    with an input or with one another are refused.
 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of

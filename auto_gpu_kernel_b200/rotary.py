@@ -67,7 +67,8 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
     """Rotate `q_pe` [n,heads,64] (bf16, strided token and head rows allowed, 1 to 128 heads) into `q_out` (contiguous;
     allocated when None; may be q_pe itself where that is contiguous) and return it; rotate `kpe` [n,64] and store it
     with `ckv` [n,512] at global slot `slots[t]` of the paged caches [P,64,512] / [P,64,64] (-1 skips the token's
-    cache rows; two equal slots race).
+    cache rows; two equal slots race).  `q_out` over any other argument and caches over one another are refused; `ckv`
+    and `kpe` may be rows of the caches that no slot of the call names.
 
     Pair i of token t turns by positions[pair_axes[i], t] * inv_freq[i]: `positions` [axes,n] int32 with one to four axes
     (rows may be expanded),
@@ -98,8 +99,6 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
         raise ValueError("rotary: q_out must be a contiguous [n,heads,64] bf16 tensor")
     elif q_out.get_device() != index:
         raise RuntimeError(f"rotary: all tensors must be on cuda:{index}")
-    elif workspace.overlap(q_out, q_pe) and not (q_out.data_ptr() == q_pe.data_ptr() and q_pe.is_contiguous()):
-        raise ValueError("rotary: q_out overlaps q_pe without being the same contiguous tensor")
     if n == 0:
         return q_out
     # the stride of an axis of one entry says nothing

@@ -67,18 +67,6 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory spans of two tensors meet (from the first element to the last, gaps included)."""
-    pa, pb = a.data_ptr(), b.data_ptr()
-    if pa == 0 or pb == 0 or a.numel() == 0 or b.numel() == 0:
-        return False
-    low, first, last = (a, pa, pb) if pa <= pb else (b, pb, pa)
-    span = 1
-    for n, s in zip(low.shape, low.stride()):
-        span += (n - 1) * s
-    return last < first + span * low.element_size()
-
-
 STATUS_BITS = {
     0x1: "a bounded device-side wait timed out",
     0x2: "block_table entry outside [0, num_pages)",

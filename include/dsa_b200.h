@@ -41,7 +41,8 @@ enum {
   DSA_ERR_WORKSPACE_TOO_SMALL = -3,
   DSA_ERR_MISALIGNED = -4,
   DSA_ERR_UNSUPPORTED = -5,
-  DSA_ERR_SCRATCH_TOO_SMALL = -6 /* dsa_indexer_topk_noalloc: batch x padded context > built-in scratch */
+  DSA_ERR_SCRATCH_TOO_SMALL = -6, /* dsa_indexer_topk_noalloc: batch x padded context > built-in scratch */
+  DSA_ERR_OVERLAP = -7 /* an output shares memory with an input or with another output */
 };
 
 /* bits OR-ed into *status_dev by kernels */
@@ -210,6 +211,7 @@ int dsa_kv_cache_append(const void* ckv, int64_t ckv_stride, const void* kpe, in
  *           buffer.  Entries at or behind seq_len are left as they were.
  *   workspace >= dsa_paged_attn_workspace_bytes(...) bytes, 256-byte aligned, any contents; calls that may
  *           overlap need workspaces of their own.
+ * An output that shares memory with an input, another output or the workspace is refused (DSA_ERR_OVERLAP).
  * max_pages, num_pages <= DSA_PAGED_MAX_PAGES; tokens_per_request * heads <= 65536.
  * ------------------------------------------------------------------------------------------- */
 #define DSA_PAGED_MAX_PAGES (1 << 24)
@@ -236,7 +238,8 @@ int dsa_paged_attn(const void* q_nope, const void* q_pe, const void* ckv, const 
  *   the last kept token 0 and -1.
  * The old pages are only read.  A new page must not be an old page that a request of the call still reads
  * from, unless every kept token on it keeps its place (a request within the budget may pass its old row and
- * nothing moves), nor stand twice in new_block_table: such moves race.  The outputs must not overlap the inputs.
+ * nothing moves), nor stand twice in new_block_table: such moves race.  An output that shares memory with an input,
+ * a cache or another output is refused (DSA_ERR_OVERLAP).
  * Page ids outside [0, num_pages) are skipped (DSA_STATUS_BAD_PAGE).
  * max_pages, num_pages <= DSA_PAGED_MAX_PAGES; budget <= DSA_EVICT_MAX_BUDGET (the tokens of as many pages).
  * ------------------------------------------------------------------------------------------- */
@@ -261,6 +264,8 @@ int dsa_cache_evict(const float* token_weights, int64_t token_weights_stride, co
  *   q_out [tokens,heads,64] bf16 contiguous (may be q_pe where that is contiguous) receives the rotated queries of
  *   every token; ckv_cache / kpe_cache [num_slots,512 / 64] receive ckv[t] and the rotated kpe[t] at slot slots[t]
  *   (-1 = not cached, as for dsa_kv_cache_append, which also says what bad and equal slots do).
+ * q_out over anything but q_pe, and caches over q_pe, positions, inv_freq, slots or one another, are refused
+ * (DSA_ERR_OVERLAP).  ckv and kpe may be rows of the caches that no slot of the call names.
  * ------------------------------------------------------------------------------------------- */
 int dsa_rotary_append(const void* q_pe, int64_t q_token_stride, int64_t q_head_stride, const void* ckv,
                       int64_t ckv_stride, const void* kpe, int64_t kpe_stride, const int32_t* positions,
