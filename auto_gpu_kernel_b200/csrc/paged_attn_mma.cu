@@ -156,7 +156,8 @@ paged_attn_mma_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_
     issue_tile();
   }
 
-  // where the logits of a tile go (only where they are wanted)
+  // where the logits of a tile go (only where they are wanted; padding rows among them: leaving these out cost 3 % at
+  // 64 x 16384 tokens x 16 rows, 223 us against 216, and gave nothing at 64 x 8192 x 5 rows)
   auto tile_logits = [&](const PaTile& t) {
     return a.logits + (((size_t)t.b * a.max_pages + t.j) * gridDim.y + rb) * (size_t)(kPaRows * kPage);
   };

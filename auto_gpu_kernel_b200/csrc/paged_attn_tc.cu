@@ -156,7 +156,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
         lim1 = row_tok[1] < 0 ? 0 : tile.len - a.tokens + 1 + row_tok[1];
       }
       const int pos0 = tile.j * kPage;
-      float* lg = nullptr;
+      float* lg = nullptr;                           // (rows behind a request's last are not stored)
       if (kLogits)
         lg = a.logits + ((((size_t)tile.b * a.max_pages + tile.j) * gridDim.y + rb) * kTcRows + row0) * (size_t)kPage +
              32 * half + 2 * t4;
@@ -218,8 +218,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
         if (kLogits && tile.len > 0) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            *reinterpret_cast<float2*>(lg + 8 * k) = make_float2(-INFINITY, -INFINITY);
-            *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * k) = make_float2(-INFINITY, -INFINITY);
+            if (row_tok[0] >= 0) *reinterpret_cast<float2*>(lg + 8 * k) = make_float2(-INFINITY, -INFINITY);
+            if (row_tok[1] >= 0) *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * k) = make_float2(-INFINITY, -INFINITY);
           }
         }
       } else {
@@ -234,8 +234,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_ckv, const __grid_c
         if (kLogits) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            *reinterpret_cast<float2*>(lg + 8 * k) = make_float2(x[4 * k], x[4 * k + 1]);
-            *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * k) = make_float2(x[4 * k + 2], x[4 * k + 3]);
+            if (row_tok[0] >= 0) *reinterpret_cast<float2*>(lg + 8 * k) = make_float2(x[4 * k], x[4 * k + 1]);
+            if (row_tok[1] >= 0) *reinterpret_cast<float2*>(lg + 8 * kPage + 8 * k) = make_float2(x[4 * k + 2], x[4 * k + 3]);
           }
         }
         if (told & 1) {

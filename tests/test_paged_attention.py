@@ -391,3 +391,32 @@ def test_refusals():
     refuses(ValueError, a0=args[0][:0], a1=args[1][:0], new_token_weights=w)          # two requests, no query token
     none = paged_attention.run(*args[:5], args[5][:, :0], SCALE)
     assert (none[0] == 0).all() and torch.isinf(none[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,tokens", [(20, 1), (5, 4), (33, 2), (64, 1), (100, 1)])
+def test_logits_of_padding_rows_are_not_stored(heads, tokens):
+    """In blocks of 64 rows the scratch rows behind a request's last query row are not written; nobody reads them."""
+    from auto_gpu_kernel_b200 import workspace
+    lib = _lib.load()
+    q_nope, q_pe, ckv, kpe, lens, table = make([300, 64, 0, 700], heads=heads, tokens=tokens, seed=70)
+    table[3, 1] = -1                                     # a page that is left out
+    batch, pages, rows = 4, table.shape[1], tokens * heads
+    block = 64
+    blocks = -(-rows // block)
+    need = lib.dsa_paged_attn_workspace_bytes(batch, tokens, heads, pages, 1)
+    scratch = torch.full((need,), 0xa5, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty_like(q_nope), torch.empty(q_nope.shape[:2], device="cuda")
+    new = torch.zeros(batch, pages * PAGE, device="cuda")
+    rc = workspace.call_on(0, lib.dsa_paged_attn, q_nope.data_ptr(), q_pe.data_ptr(), ckv.data_ptr(), kpe.data_ptr(), lens.data_ptr(),
+                           table.data_ptr(), pages, SCALE, out.data_ptr(), lse.data_ptr(), None, 0, new.data_ptr(), pages * PAGE, batch,
+                           tokens, heads, ckv.shape[0], pages, scratch.data_ptr(), need)
+    assert rc == 0
+    with pytest.raises(RuntimeError, match="block_table entry outside"):
+        workspace.check_status()
+    logits = scratch[need - 4 * batch * pages * blocks * block * PAGE:].view(torch.int32).view(batch, pages, blocks * block, PAGE)
+    untouched = logits == -0x5a5a5a5b                    # bytes 0xa5
+    assert untouched[:, :, rows:].all()
+    for b, n in enumerate(lens.tolist()):
+        held = -(-n // PAGE)
+        assert not untouched[b, :held, :rows].any() and untouched[b, held:].all()
