@@ -23,6 +23,15 @@ def sections(*counts):
     return [axis for axis, n in enumerate(counts) for _ in range(n)]
 
 
+def _axis_bytes(pair_axes):
+    """A byte per pair, from any sequence of whole numbers (by way of a list: bytes() of an array would be its buffer, of a
+    number as many zeros)."""
+    try:
+        return bytes(list(pair_axes))
+    except TypeError:
+        raise ValueError(f"rotary: pair_axes must be {PAIRS} axis numbers") from None
+
+
 @functools.lru_cache(maxsize=64)
 def _pack(pair_axes, axes):
     """The axes (a byte per pair) in two bits each."""
@@ -77,8 +86,6 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
     index, bf16 = q_pe.get_device(), torch.bfloat16
     shape = q_pe.shape
     n = shape[0] if len(shape) == 3 else -1
-    if isinstance(pair_axes, int):
-        raise ValueError(f"rotary: pair_axes must be {PAIRS} axis numbers")
     if not (index >= 0 and len(shape) == 3 and shape[2] == 64 and 1 <= shape[1] <= 128 and q_pe.dtype is bf16
             and q_pe.stride(2) == 1 and ckv.shape == (n, 512) and kpe.shape == (n, 64) and ckv.dtype is bf16
             and kpe.dtype is bf16 and ckv.stride(1) == 1 and kpe.stride(1) == 1
@@ -92,7 +99,7 @@ def append(q_pe, ckv, kpe, positions, inv_freq, pair_axes, slots, ckv_cache, kpe
             == ckv_cache.get_device() == kpe_cache.get_device() == index):
         _refuse(q_pe, ckv, kpe, positions, inv_freq, slots, ckv_cache, kpe_cache)
     heads, axes, num_slots = shape[1], positions.shape[0], ckv_cache.numel() // 512
-    packed = _pack(bytes(pair_axes), axes)
+    packed = _pack(_axis_bytes(pair_axes), axes)
     if q_out is None:
         q_out = q_pe.new_empty((n, heads, 64))
     elif q_out.shape != shape or q_out.dtype is not bf16 or not q_out.is_contiguous():

@@ -58,6 +58,20 @@ def test_sections():
             rotary.sections(*bad)
 
 
+def test_pair_axes_of_any_sequence():
+    import numpy as np
+    want = rotary._pack(bytes(rotary.sections(16, 8, 8)), 3)
+    axes = rotary.sections(16, 8, 8)
+    for form in (axes, tuple(axes), bytes(axes), np.array(axes), np.array(axes, dtype=np.int8), torch.tensor(axes)):
+        assert rotary._pack(rotary._axis_bytes(form), 3) == want, type(form)
+    for bad in (32, None, [0.0] * 32, np.zeros(32), [-1] * 32, [256] * 32):
+        with pytest.raises(ValueError):
+            rotary._axis_bytes(bad)
+    for bad in (np.zeros(4, dtype=np.int64), np.zeros(64, dtype=np.int8), [0] * 31, [3] * 32, range(0)):
+        with pytest.raises(ValueError):                  # (the buffer of four 64-bit numbers has 32 bytes)
+            rotary._pack(rotary._axis_bytes(bad), 3)
+
+
 def test_host_side_argument_errors():
     f = _lib.load().dsa_rotary_append
     ok = dict(q=16, qt=1024, qh=64, c=16, cs=512, k=16, ks=64, p=16, ps=4, axes=2, f=16, pa=0x5555, i=1, s=16, o=16, cc=16, kc=16,
@@ -206,3 +220,15 @@ def test_refusals():
     empty = {**case, "q_pe": q[:0], "ckv": case["ckv"][:0], "kpe": case["kpe"][:0], "positions": case["positions"][:, :0],
              "slots": case["slots"][:0]}
     assert rotary.append(**empty).shape == (0, 16, 64)
+
+
+@pytest.mark.gpu
+def test_pair_axes_as_an_array():
+    import numpy as np
+    case = make(20, axes=3, seed=9)
+    want = rotary.append(**case)
+    case["pair_axes"] = np.array(case["pair_axes"])
+    assert torch.equal(rotary.append(**case), want)
+    for bad in (np.zeros(4, dtype=np.int64), 32, None):
+        with pytest.raises(ValueError, match="pair_axes"):
+            rotary.append(**{**case, "pair_axes": bad})
