@@ -36,7 +36,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 
 _NO_GUARD = contextlib.nullcontext()
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# cudaStream_t of the current stream of the device with this index
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def device_guard(device: torch.device):
@@ -62,7 +63,7 @@ def call_on(index: int, fn, *args) -> int:
 
 def stream_handle(device: torch.device) -> int:
     """cudaStream_t of torch's current stream on `device` (the stream the C ABI enqueues on)."""
-    if _raw_stream is not None and device.index is not None:
+    if device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
