@@ -449,17 +449,26 @@ static bool paged_shape_ok(int batch, int tokens, int heads, int max_pages) {
   return batch >= 0 && batch <= 65535 && tokens >= 1 && heads >= 1 && heads <= 128 && (int64_t)tokens * heads <= 65536 &&
          max_pages >= 1 && max_pages <= DSA_PAGED_MAX_PAGES;
 }
-// Whether requests stay whole, from the batch and the width of the block table (the lengths are on the device).  With f
-// CTAs' worth of requests per SM and p pages each, a CTA that takes whole requests is done after ceil(f) of them, about
-// 1.6 p + 3.5 us each; cut ones take f (1.6 p + 5) us, and 10 us for partial results and their join.  The second
-// condition bounds what is lost where most requests are much shorter than the table.  Measured, cut / whole, 16 rows:
-// 1 x 2 pages 11.0 / 9.0 us, 1 x 6 12.3 / 15.8, 64 x 8 22.6 / 20.5, 64 x 16 28.8 / 32.8, 148 x 8 34.2 / 22.6, 160 x 16 53 / 62,
-// 300 x 4 51 / 35, 700 x 8 135 / 86; lengths of 1 to p pages: 160 x 16 32 / 39, 300 x 16 50 / 43, 700 x 24 105 / 84.
+// Whether requests stay whole, from the batch and the width of the block table (the lengths are on the device).  Whole ones
+// save a launch, the partial results and their join; cut ones spread the pages evenly.  The widest table that is better left
+// whole grows with the requests (times row blocks) per SM: 3 pages and 13.5 more for each while every one has an SM of
+// its own, 2 and 8.5 more beyond, where the last turn leaves SMs idle.  Fitted to the geometric mean over three kinds of
+// lengths (all of the table, evenly spread over 1 .. table, spread over its logarithm), 227 pairs of batch and table
+// of 16, 64 and 128 rows; the rule takes the slower side by more than 4 % twice (7 % at most: 64 rows, 8 x 4 pages).
+// Measured, cut / whole in us, calls in a graph, caches larger than L2; all of the table, even, logarithm:
+//   left whole  16 rows:   32 x 4 pages  13.3/11.2  12.8/11.2  11.8/11.0     64 rows:   32 x 4   19.2/14.6  17.7/14.6  15.2/14.5
+//                         100 x 12       31.5/25.2  25.8/24.5  20.4/22.4               100 x 12  38.6/31.0  30.3/30.4  23.9/27.6
+//                         160 x 8        36.8/35.4  30.9/27.3  27.6/21.8               160 x 8   45.7/44.6  37.3/32.9  32.1/27.4
+//                         300 x 16       87.8/88.4  61.5/57.4  48.5/41.3               300 x 16   101/102   76.8/71.2  57.3/48.1
+//                         700 x 16        191/147    136/105   95.9/61.7               700 x 16   223/170    168/132    116/79.6
+//   cut         16 rows:   32 x 8 pages  15.4/17.3  13.7/17.4  11.0/12.7     64 rows:   64 x 12  29.2/29.2  24.1/28.9  21.2/26.9
+//                         100 x 16       35.0/31.3  27.5/30.8  22.0/28.8               100 x 16  45.3/37.5  34.9/37.1  25.9/34.6
+//                         160 x 12       44.5/47.7  34.3/33.7  27.6/30.1               160 x 12  54.9/58.1  41.7/43.8  32.4/36.2
+//                         300 x 24        113/126   75.7/85.1  51.0/55.6               300 x 24   129/143   91.7/94.6  60.2/60.0
 static int paged_split(int batch, int blocks, int max_pages) {
-  const int sms = dsa::sm_count();
-  const int64_t ctas = (int64_t)batch * blocks;
-  const double f = (double)ctas / sms, turns = (double)((ctas + sms - 1) / sms);
-  if (max_pages > 8 + 5 * f || 1.6 * max_pages * (turns - f) > 5 * f - 3.5 * turns + 10) return dsa::kPagedCut;
+  const int64_t sms = dsa::sm_count(), ctas = (int64_t)batch * blocks;
+  const int64_t widest = ctas <= sms ? (6 * sms + 27 * ctas) / (2 * sms) : (4 * sms + 17 * ctas) / (2 * sms);
+  if (max_pages > widest) return dsa::kPagedCut;
   return ctas <= sms ? dsa::kPagedOne : dsa::kPagedSnap;
 }
 // Ranges that the tiles are cut into: a CTA per SM over all row blocks, so that the blocks of one request walk its

@@ -93,6 +93,25 @@ def test_workspace_holds_partials_and_logits():
     assert size(1, 4096, 16, 512, 0) == 256                # nor do more row blocks than SMs
 
 
+@pytest.mark.parametrize("rows", [16, 64, 128])
+def test_requests_are_cut_where_that_was_measured_to_be_faster(rows):
+    """The plan shows in the workspace: whole requests leave no partial results.  148 SMs; requests, pages of the table, and
+    whether whole ones took less time in the geometric mean over full, evenly and logarithmically spread lengths."""
+    size = _lib.load().dsa_paged_attn_workspace_bytes
+    measured = {
+        16: [(1, 2, True), (1, 8, False), (8, 8, False), (32, 4, True), (32, 8, False), (64, 4, True), (64, 12, False), (100, 12, True),
+             (100, 16, False), (148, 16, True), (148, 24, False), (160, 8, True), (160, 12, False), (200, 12, True), (200, 16, False),
+             (300, 8, True), (300, 16, True), (300, 24, False), (450, 16, True), (450, 24, True), (700, 16, True), (1000, 12, True)],
+        64: [(1, 2, True), (1, 8, False), (8, 8, False), (32, 4, True), (32, 12, False), (64, 4, True), (64, 12, False), (100, 12, True),
+             (100, 16, False), (148, 16, True), (148, 24, False), (160, 8, True), (160, 12, False), (200, 12, True), (200, 16, False),
+             (300, 16, True), (300, 24, False), (450, 16, True), (450, 24, True), (700, 16, True)],
+        128: [(1, 2, True), (1, 8, False), (8, 4, True), (8, 8, False), (32, 8, True), (32, 12, False), (64, 12, True), (64, 24, False),
+              (100, 12, True), (100, 16, False), (148, 16, True), (148, 32, False), (160, 16, True), (160, 32, False), (200, 16, True),
+              (300, 24, True), (450, 24, True), (700, 16, True)]}
+    for batch, pages, whole in measured[rows]:
+        assert (size(batch, 1, rows, pages, 0) == -(-8 * batch // 256) * 256) == whole, (batch, pages)
+
+
 def test_cpu_tensors_are_refused():
     from auto_gpu_kernel_b200 import paged_attention
     args = make([70, 5], device="cpu")
