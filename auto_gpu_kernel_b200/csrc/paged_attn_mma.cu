@@ -16,8 +16,11 @@
 //   S = Q.K^T   warp w has tokens 8w .. 8w+7 of the page; q_nope stays in registers as 32 A fragments, q_pe in shared
 //               memory (all 36 in registers left the loop none to schedule in);
 //   softmax     base 2, the running maximum refreshed (and O rescaled) only when a logit exceeds it by more than 2^8;
-//               P is rounded to bf16 for the second product, as the cache that it multiplies is bf16; sums are taken
-//               of the fp32 values;
+//               P is rounded to bf16 for the second product, whose operands have one type and whose other one is the bf16
+//               cache; sums are taken of the fp32 values.  The rounding is independent from key to key and of the size of
+//               the output's own (rms error against 64 bits 0.0020 with both, 0.0017 with the output's alone: 1 x 1000 tokens).
+//               P as a sum of two bf16 operands gives 0.0017 and makes 256 products more per page: 64 x 32768 tokens 424 -> 476 us,
+//               48 ragged requests 34.7 -> 38.1, 1 x 131071 35.6 -> 38.8, so it is not done;
 //   O += P.V    warp w has the output columns 64w .. 64w+63 = column block w of the same stage (ldmatrix.trans).
 // Rows behind a request's length are put to zero in the stage before the second product: the cache may hold anything
 // there, and 0 x NaN would get into the sum.

@@ -7,7 +7,9 @@
 // The first product has the rows as M: a softmax warp then holds 16 rows x 32 tokens in the fragment order of the warp-level
 // products, and writes P as that order's 4-byte pairs without bank conflicts.  The second is transposed because the
 // rows are too few for M: 512 output columns are four M = 128 blocks, and the accumulator is 256 of the 512 TMEM
-// columns, which leaves room for two S buffers.
+// columns, which leaves room for two S buffers.  P is rounded to bf16, as in paged_attn_mma.cu (which has the error and what the
+// remainder as a second operand costs; here that would be 16 more instructions of 49 cycles per page, and 8 KB of shared
+// memory beside q and two pages, where less than 2 KB are left); the sums are taken of the fp32 values.
 //
 // Bounds: an instruction reads its operands from shared memory at 128 B per cycle, so the first product's cost 32 cycles
 // (M = N = 64; measured 36 when a converged warp issues them, 55-160 from a branch of one lane, whose descriptors have

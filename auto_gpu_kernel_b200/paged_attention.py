@@ -163,7 +163,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     heads).  `seq_lens` counts the cached tokens of each request, the new ones among them: token i of n sees the
     positions below seq_len - n + 1 + i, and one that sees none gets output 0 and lse -inf.  Cache rows at or
     behind seq_len may hold anything, those in front of it must be finite.  Outputs that share memory
-    with an input or with one another are refused.
+    with an input or with one another are refused.  Logits, sums, lse and accumulated weights are fp32; the softmax weights
+    are rounded to bf16 for their product with the bf16 cache, an error of the size of the output's own rounding.
 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
