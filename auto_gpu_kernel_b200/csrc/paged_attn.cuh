@@ -44,8 +44,9 @@ enum PagedSplit {
 
 // Query rows that a CTA takes at once, from the rows of a request: 16 by warp-level products, 64 by tcgen05.  At 16 rows the
 // first keeps three pages in shared memory where the second has room for two beside its q (64 x 32768 tokens 363 us
-// against 411 us, 1 x 131071 37 us against 53 us); from 17 rows on the second reads the cache once where the first would
-// read it for every 16 (32 rows, 64 x 8192 tokens: 118 us, and 154 us for warp-level products with two row groups).
+// against 411 us in runs of a few ms, 1 x 131071 37 us against 53 us); from 17 rows on the second reads the cache once where
+// the first would read it for every 16 (32 rows, 64 x 8192 tokens: 118 us, and 154 us for warp-level products with two row
+// groups).
 inline int paged_block_rows(int rows) { return rows <= 16 ? 16 : 64; }
 // What taking up a request costs, in tiles (48 requests of 1 to 16384 tokens, 16 rows: cost 0 / 1 / 2 / 3 / 4 60 / 45 / 41.5 /
 // 40.9 / 43.3 us; 64 rows are flat from 2 on, 200 short requests best at 2).

@@ -169,7 +169,8 @@ def kernel(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, 
     `new_token_weights` [B,>= 64*max_pages] float32 receives, for every position below seq_len, `token_weights` (same
     shape; None = zeros; may be the same tensor) plus the softmax weight the position got from all query rows of
     its request; other entries stay as they were.  The call's scratch then holds the logits, 256 bytes per query row
-    and page of the table, so a table much wider than its lengths costs memory."""
+    and page of the table, so a table much wider than its lengths costs memory (calls on a few requests at a time hold
+    less at once)."""
     if output is None or lse is None:
         raise ValueError("paged attention: kernel() needs output and lse")
     _attend(q_nope, q_pe, ckv_cache, kpe_cache, seq_lens, block_table, sm_scale, output, lse, token_weights, new_token_weights)
