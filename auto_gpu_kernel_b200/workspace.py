@@ -26,7 +26,9 @@ def get(device: torch.device, purpose: str, nbytes: int) -> torch.Tensor:
 
 
 def status_word(device: torch.device) -> torch.Tensor:
-    """The int32 word kernels OR their DSA_STATUS_* bits into."""
+    """The int32 word kernels OR their DSA_STATUS_* bits into.  The first call on a device allocates and zeroes it; made
+    inside a stream capture, the zeroing would become part of the graph, and each replay would forget the bits that
+    nobody has read yet, so make one call (or this one) before capturing."""
     key = device.index if device.index is not None else torch.cuda.current_device()
     word = _status.get(key)
     if word is None:
